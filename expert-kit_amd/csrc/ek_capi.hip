@@ -1,10 +1,10 @@
 // C-ABI host layer of libek_hip.so (see include/ek_hip.h for the contract).
 #include "../../include/ek_hip.h"
+#include "ek_host.h"
 #include "ek_internal.h"
 
 #include <algorithm>
 #include <chrono>
-#include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -27,51 +27,11 @@ void set_last_error(const char *msg) { g_last_error = msg ? msg : ""; }
 
 namespace {
 
-ek_status fail(ek_status st, const char *fmt, ...)
-{
-    char buf[512];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    g_last_error = buf;
-    return st;
-}
-
-ek_status hip_fail(hipError_t e, const char *what)
-{
-    (void)hipGetLastError();   // clear the sticky error
-    return fail(e == hipErrorOutOfMemory ? EK_OOM : EK_HIP_ERROR, "%s: %s", what,
-                hipGetErrorString(e));
-}
-
-#define EK_HIP(call)                                                  \
-    do {                                                              \
-        hipError_t _e = (call);                                       \
-        if (_e != hipSuccess) return hip_fail(_e, #call);             \
-    } while (0)
-
-#define EK_TRY(call)                                                  \
-    do {                                                              \
-        ek_status _s = (call);                                        \
-        if (_s != EK_OK) return _s;                                   \
-    } while (0)
-
-// Makes `dev` current for the scope and restores the caller's device.
-struct DeviceGuard {
-    int prev = -1;
-    bool ok = false;
-    explicit DeviceGuard(int dev)
-    {
-        if (hipGetDevice(&prev) != hipSuccess) { (void)hipGetLastError(); prev = -1; }
-        ok = hipSetDevice(dev) == hipSuccess;
-        if (!ok) (void)hipGetLastError();
-    }
-    ~DeviceGuard()
-    {
-        if (prev >= 0 && ok) (void)hipSetDevice(prev);
-    }
-};
+using ek::DeviceGuard;
+using ek::WorkspaceUse;
+using ek::dev_alloc;
+using ek::fail;
+using ek::hip_fail;
 
 int64_t elem_size(int dt)
 {
@@ -233,18 +193,6 @@ constexpr int64_t kSharedStreamRows = 64, kSharedWideRows = 256;
 constexpr int64_t kSharedWideItems = kSharedWideRows / ek::kWideRows;
 
 ek_status static_scratch_setup(int dev);   // (defined with ek_layer_forward_static's scratch array)
-
-ek_status dev_alloc(void **p, size_t bytes, const char *what)
-{
-    hipError_t e = hipMalloc(p, bytes ? bytes : 16);
-    if (e != hipSuccess) {
-        *p = nullptr;
-        (void)hipGetLastError();
-        return fail(e == hipErrorOutOfMemory ? EK_OOM : EK_HIP_ERROR, "hipMalloc(%s, %zu bytes): %s",
-                    what, bytes, hipGetErrorString(e));
-    }
-    return EK_OK;
-}
 
 void free_layer(ek_layer *L)
 {
@@ -684,39 +632,6 @@ ek_status set_expert_padded(ek_layer *L, int32_t e, const ek_weight_desc *up, co
     g_last_error = keep;
     return st;
 }
-
-// One use of a layer's workspace on stream s; the caller holds L->mu for the scope.
-// begin(): the stream waits (on the device) for the last enqueue-only call that used the
-// workspace.  At the end of the scope the stream's position is recorded as that call's end,
-// unless synced() says the host has waited for the stream, after which nothing is pending.
-// A stream under capture by the caller is left alone both ways (a captured wait on an event
-// recorded outside the capture is not allowed): replays of such a graph use the workspace like
-// the call they record, and ordering them against other calls on the layer is the caller's part.
-struct WorkspaceUse {
-    hipEvent_t ev;
-    bool *busy;
-    hipStream_t s;
-    bool capturing = false, host_synced = false;
-    WorkspaceUse(ek_layer *layer, hipStream_t stream) : ev(layer->ev_ws), busy(&layer->ws_busy), s(stream) {}
-    WorkspaceUse(hipEvent_t event, bool *busy_flag, hipStream_t stream) : ev(event), busy(busy_flag), s(stream) {}
-    ek_status begin()
-    {
-        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(s, &cs) != hipSuccess) { (void)hipGetLastError(); cs = hipStreamCaptureStatusNone; }
-        capturing = cs != hipStreamCaptureStatusNone;
-        if (!capturing && *busy) EK_HIP(hipStreamWaitEvent(s, ev, 0));
-        return EK_OK;
-    }
-    void device_idle() { *busy = false; }          // after a hipDeviceSynchronize
-    void synced() { host_synced = true; }          // after a hipStreamSynchronize(s) that followed begin()
-    ~WorkspaceUse()
-    {
-        if (capturing) return;
-        if (host_synced) { *busy = false; return; }
-        if (hipEventRecord(ev, s) == hipSuccess) *busy = true;
-        else (void)hipGetLastError();
-    }
-};
 
 // ---- ek_layer_forward_static: the workspace of a layer call in a static device array ----------
 // Callers that must not allocate (code under HIP graph capture, serving loops, harnesses that
@@ -1307,17 +1222,6 @@ ek_status finish_blocking(ek_layer *L, const Workspace &W, hipStream_t s)
 
 // ------------------------------------------------------------------ C ABI
 
-#define EK_GUARDED(...)                                               \
-    try {                                                             \
-        __VA_ARGS__                                                   \
-    } catch (const std::bad_alloc &) {                                \
-        return fail(EK_OOM, "host allocation failed");                \
-    } catch (const std::exception &ex) {                              \
-        return fail(EK_INTERNAL, "exception: %s", ex.what());         \
-    } catch (...) {                                                   \
-        return fail(EK_INTERNAL, "unknown exception");                \
-    }
-
 extern "C" {
 
 const char *ek_backend_name(void) { return "hip"; }
@@ -1436,7 +1340,7 @@ ek_status ek_layer_forward(ek_layer *layer, const void *x, const int32_t *ids, c
         const int w_f32 = w_dtype == EK_F32;
         std::lock_guard<std::mutex> lk(layer->mu);
         hipStream_t s = stream ? (hipStream_t)stream : layer->stream;
-        WorkspaceUse use(layer, s);
+        WorkspaceUse use(layer->ev_ws, &layer->ws_busy, s);
         EK_TRY(use.begin());
         ek_status st = EK_OK;
         // a blocking call on device buffers sees everything submitted before it
@@ -1517,7 +1421,7 @@ ek_status ek_layer_forward_static(ek_layer *layer, const void *x, const int32_t 
         std::lock_guard<std::mutex> lk(layer->mu);      // the layer's side stream, events and slab table
         std::lock_guard<std::mutex> sk(S.mu);           // the device's scratch array
         hipStream_t s = stream ? (hipStream_t)stream : layer->stream;
-        WorkspaceUse use(layer, s);
+        WorkspaceUse use(layer->ev_ws, &layer->ws_busy, s);
         EK_TRY(use.begin());
         WorkspaceUse use_scratch(S.ev, &S.busy, s);
         EK_TRY(use_scratch.begin());
@@ -1560,7 +1464,7 @@ ek_status ek_layer_pack(ek_layer *layer, const int32_t *ids, int64_t T, const ek
         const int64_t H = layer->user_hidden, K = layer->cfg.top_k, P = T * K;   // rows are gathered as the caller has them
         std::lock_guard<std::mutex> lk(layer->mu);
         hipStream_t s = stream ? (hipStream_t)stream : layer->stream;
-        WorkspaceUse use(layer, s);
+        WorkspaceUse use(layer->ev_ws, &layer->ws_busy, s);
         EK_TRY(use.begin());
         if (mem == EK_DEVICE && !stream) { EK_HIP(hipDeviceSynchronize()); use.device_idle(); }
         const int32_t *d_ids = ids;
@@ -1611,7 +1515,7 @@ ek_status ek_layer_expert_forward(ek_layer *layer, int32_t expert, const void *x
         if (!layer->expert_mem[expert])
             return fail(EK_EXPERT_NOT_FOUND, "expert %d is not loaded", expert);
         hipStream_t s = stream ? (hipStream_t)stream : layer->stream;
-        WorkspaceUse use(layer, s);
+        WorkspaceUse use(layer->ev_ws, &layer->ws_busy, s);
         EK_TRY(use.begin());
         if (mem == EK_DEVICE && !stream) { EK_HIP(hipDeviceSynchronize()); use.device_idle(); }
         if (n > 0) {
@@ -1697,7 +1601,7 @@ ek_status ek_layer_experts_forward(ek_layer *layer, int32_t n_calls, const int32
             if (!layer->expert_mem[experts[i]])
                 return fail(EK_EXPERT_NOT_FOUND, "expert %d is not loaded", experts[i]);
         hipStream_t s = stream ? (hipStream_t)stream : layer->stream;
-        WorkspaceUse use(layer, s);
+        WorkspaceUse use(layer->ev_ws, &layer->ws_busy, s);
         EK_TRY(use.begin());
         if (mem == EK_DEVICE && !stream) { EK_HIP(hipDeviceSynchronize()); use.device_idle(); }
         if (P > 0) {
@@ -2120,7 +2024,7 @@ ek_status ek_chain_forward(ek_chain *chain, const void *x, const int32_t *ids, c
         // every layer's workspace is used on s: eagerly, or by the replay of the graph
         std::vector<std::unique_ptr<WorkspaceUse>> uses;
         for (ek_layer *ly : order) {
-            uses.emplace_back(new WorkspaceUse(ly, s));
+            uses.emplace_back(new WorkspaceUse(ly->ev_ws, &ly->ws_busy, s));
             EK_TRY(uses.back()->begin());
         }
         const int w_f32 = w_dtype == EK_F32;
@@ -2326,7 +2230,7 @@ ek_status route_and_forward(ek_layer *layer, const void *x, const void *logits, 
     const size_t l_bytes = (size_t)T * E * (rcfg->logits_dtype == EK_F32 ? 4 : 2);
     std::lock_guard<std::mutex> lk(layer->mu);
     hipStream_t s = stream ? (hipStream_t)stream : layer->stream;
-    WorkspaceUse use(layer, s);
+    WorkspaceUse use(layer->ev_ws, &layer->ws_busy, s);
     EK_TRY(use.begin());
     if (mem == EK_DEVICE && !stream) { EK_HIP(hipDeviceSynchronize()); use.device_idle(); }
     EK_TRY(ensure_router_ws(layer, mem == EK_HOST));

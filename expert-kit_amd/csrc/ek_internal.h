@@ -198,6 +198,48 @@ hipError_t launch_ffn_tile(const FfnArgs &a, int stage, int act, int wmode,
 // hidden channels (stage 1) / output channels (stage 2) per tile workgroup
 constexpr int tile_channels(int stage, bool narrow) { return (stage == 1 ? 256 : 512) / (narrow ? 2 : 1); }
 
+// ---- 8-bit activations ----------------------------------------------------------
+// Rows of 16-bit values -> int8 rows and one scale per row, with (norm) the residual's addition and the
+// RMS norm in front: see ek_quant.hip for the definition.
+struct RowQuantArgs {
+    const void *x;            // [n, H] activation type
+    const void *residual;     // [n, H] or nullptr (norm)
+    const void *gain;         // [H] (norm)
+    void *sum;                // [n, H] or nullptr: x + residual (norm)
+    void *y;                  // [n, H] or nullptr: the normed rows (norm)
+    uint8_t *q;               // [n, q_stride] int8 or nullptr; columns H .. q_stride-1 are set to zero
+    float *scale;             // [n] or nullptr
+    int64_t n;
+    int32_t H;                // norm: a multiple of 8
+    int32_t q_stride;         // a multiple of 8, at least H
+    float eps;
+    double inv_h;             // 1 / H
+    bool vec;                 // rows of x start on 16-byte boundaries (H a multiple of 8)
+};
+hipError_t launch_row_quant(const RowQuantArgs &a, int act, bool norm, hipStream_t s);
+// int8 rows of len bytes back to back -> rows of `stride` bytes with a zero tail
+hipError_t launch_pad_rows8(const void *src, int64_t n, int32_t len, void *dst, int32_t stride, hipStream_t s);
+
+// Products of int8 rows with int8 weights (per-channel scales): ek_ffn_q8.hip
+struct Q8Args {
+    const uint8_t *x;         // int8 rows, stride Kdim bytes
+    const float *x_scale;     // one per row of x
+    const int32_t *rows;      // packed position -> row of x, or nullptr (identity)
+    const ExpertSlab *slabs;
+    void *out;                // stage 1: h; stage 2: output rows (packed order), activation type
+    int64_t out_stride;
+    int32_t N;                // output channels stored (stage 1: a multiple of 16)
+    int32_t NT;               // 16-channel tiles the weights hold
+    int32_t Kdim;             // a multiple of 64
+    const float *bias;        // [N] or nullptr (stage 2)
+    WorkLists lists;          // dense calls (one matrix, rows 0 .. n-1): items[] unused
+    int64_t dense_rows = 0;   // > 0: a dense call of that many rows on slab 0
+};
+// stage 1: up/gate + SwiGLU; stage 2: one matrix.  max_items[l]: bound of list l (see launch_ffn_tile);
+// wide: the streaming list holds items of up to kWideRows rows
+hipError_t launch_ffn_q8(const Q8Args &a, int stage, int act, const int64_t max_items[kNumLists], bool wide, hipStream_t s);
+hipError_t launch_dense_q8(const Q8Args &a, int act, hipStream_t s);
+
 // ---- combine ----------------------------------------------------------------
 struct CombineArgs {
     const void *yp;           // [P, H] packed expert outputs

@@ -69,6 +69,16 @@ class ek_router_cfg(ctypes.Structure):
                 ("logits_dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32), ("bias", ctypes.c_void_p)]
 
 
+class ek_norm_cfg(ctypes.Structure):
+    _fields_ = [("hidden", ctypes.c_int64), ("act_dtype", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("device_id", ctypes.c_int32), ("flags", ctypes.c_int32)]
+
+
+class ek_linear_cfg(ctypes.Structure):
+    _fields_ = [("in_features", ctypes.c_int64), ("out_features", ctypes.c_int64), ("max_rows", ctypes.c_int64),
+                ("act_dtype", ctypes.c_int32), ("device_id", ctypes.c_int32), ("flags", ctypes.c_int32)]
+
+
 (EK_ROUTER_SOFTMAX_TOPK, EK_ROUTER_TOPK_RAW, EK_ROUTER_TOPK_SOFTMAX, EK_ROUTER_TOPK_SIGMOID,
  EK_ROUTER_SIGMOID_GROUP) = range(5)
 EK_ROUTER_MASK_NEG_INF = 1
@@ -131,6 +141,14 @@ PROTOTYPES = {
     "ek_expert_forward": (_I32, [_P, _P, _I64, _P, _I32, _P]),
     "ek_expert_shape": (_I32, [_P, ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
     "ek_expert_destroy": (_I32, [_P]),
+    "ek_norm_create": (_I32, [ctypes.POINTER(ek_norm_cfg), _P, _I32, _PP]),
+    "ek_norm_forward": (_I32, [_P, _P, _P, _I64, _P, _P, _P, _P, _I32, _P]),
+    "ek_norm_shape": (_I32, [_P, ctypes.POINTER(_I64), ctypes.POINTER(_I32)]),
+    "ek_norm_destroy": (_I32, [_P]),
+    "ek_linear_create": (_I32, [ctypes.POINTER(ek_linear_cfg), _DESC, _P, _I32, _PP]),
+    "ek_linear_forward": (_I32, [_P, _P, _P, _I64, _P, _I32, _P]),
+    "ek_linear_shape": (_I32, [_P, ctypes.POINTER(_I64), ctypes.POINTER(_I64)]),
+    "ek_linear_destroy": (_I32, [_P]),
 }
 
 _LIB = None

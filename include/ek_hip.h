@@ -482,6 +482,66 @@ ek_status ek_expert_forward(ek_expert *expert, const void *x, int64_t n, void *o
 ek_status ek_expert_shape(ek_expert *expert, int64_t *hidden, int64_t *inter);
 ek_status ek_expert_destroy(ek_expert *expert);
 
+/* ---- 8-bit activations (W8A8) ------------------------------------------------
+ * The reference computes on 16-bit activations only (its W8A16 path dequantises the weights:
+ * ffn/expert_torch.rs:24-53); checkpoints quantised to W8A8 hold int8 weights with one scale per
+ * output channel and expect every activation row quantised with one scale of its own:
+ *   q = rint(127 v / max|v|) (ties to even),  scale = max|v| / 127,  v ~ q * scale
+ * (a row of zeros has scale 0; a row that holds an infinity or NaN has q = 0 and scale NaN).
+ * Three kinds of object compute on such rows: ek_norm makes them, ek_linear multiplies them with one
+ * matrix, and a layer created with EK_CFG_ACT8 runs its experts on them. */
+
+/* RMS norm of the residual stream, in front of an MoE block (and of attention):
+ *   sum = rnd16(x + residual)           (x itself when residual is NULL)
+ *   v   = sum * gain / sqrt(mean(sum^2) + eps)
+ *   y   = rnd16(v)                      for the router's gate product and other 16-bit readers
+ *   q, scale = v quantised as above     (from v itself, not from y)
+ * rnd16 is the rounding to act_dtype; nothing else is rounded to 16 bits.  q is exactly the definition's
+ * (the scale cancels rstd out of it), whatever the order of the sum over the row. */
+typedef struct ek_norm ek_norm;
+typedef struct ek_norm_cfg {
+    int64_t hidden;      /* row length: a positive multiple of 8 */
+    int32_t act_dtype;   /* EK_BF16 or EK_F16: x, residual, gain, sum and y */
+    float eps;           /* positive */
+    int32_t device_id;
+    int32_t flags;       /* 0 */
+} ek_norm_cfg;
+/* gain: [hidden] of act_dtype, copied. */
+ek_status ek_norm_create(const ek_norm_cfg *cfg, const void *gain, int32_t gain_mem, ek_norm **out);
+/* x, residual [n, hidden] -> sum, y [n, hidden], q [n, hidden] int8, scale [n] fp32, n at most 65535 * 64.  residual may be
+ * NULL; so may any output (q and scale together, sum only with a residual).  sum may be x or
+ * residual, and so may y (not both the same buffer): the residual stream can be updated in place.  Device
+ * tensors are 16-byte aligned (q 8, scale 4).  With a stream the call only enqueues one kernel; calls
+ * share nothing but the gain and may overlap. */
+ek_status ek_norm_forward(ek_norm *norm, const void *x, const void *residual, int64_t n, void *sum, void *y, void *q,
+                          float *scale, int32_t mem, void *stream);
+ek_status ek_norm_shape(ek_norm *norm, int64_t *hidden, int32_t *act_dtype);
+ek_status ek_norm_destroy(ek_norm *norm);
+
+/* One int8 matrix with a scale per output channel on 8-bit activations (the projections around an MoE
+ * block, dense FFN layers):
+ *   y[i, c] = rnd16((sum_k q[i, k] w[c, k]) * (x_scale[i] * w_scale[c]) + bias[c])
+ * with the sum exact in int32 and the rest in fp32. */
+typedef struct ek_linear ek_linear;
+typedef struct ek_linear_cfg {
+    int64_t in_features;   /* 1 .. 131072 (the int32 sums cannot overflow); multiples of 64, at least 128,
+                              are read where they lie, other lengths through the workspace */
+    int64_t out_features;  /* any positive number up to 2^24 */
+    int64_t max_rows;      /* largest n a call will pass (sizes the workspace), at most 65535 * 64 */
+    int32_t act_dtype;     /* EK_BF16 or EK_F16: y, and x where x_scale is NULL */
+    int32_t device_id;
+    int32_t flags;         /* 0 */
+} ek_linear_cfg;
+/* w: [out_features, in_features] EK_I8 with EK_SCALE_PER_CHANNEL; bias: [out_features] of bias_dtype
+ * (EK_BF16, EK_F16, EK_F32), in w->mem, or NULL. */
+ek_status ek_linear_create(const ek_linear_cfg *cfg, const ek_weight_desc *w, const void *bias, int32_t bias_dtype, ek_linear **out);
+/* x [n, in_features] int8 with x_scale [n], or of act_dtype with x_scale NULL (the library quantises the
+ * rows first) -> y [n, out_features].  Device tensors are 16-byte aligned.  Calls that go through the
+ * workspace are ordered on the device like a layer's; the others share nothing and may overlap. */
+ek_status ek_linear_forward(ek_linear *linear, const void *x, const float *x_scale, int64_t n, void *y, int32_t mem, void *stream);
+ek_status ek_linear_shape(ek_linear *linear, int64_t *in_features, int64_t *out_features);
+ek_status ek_linear_destroy(ek_linear *linear);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,57 @@
+"""The definitions of the 8-bit activation path in 64 bits, on the CPU, and the tolerances that follow
+from the kernels' roundings."""
+import torch
+
+U32 = 2.0 ** -24          # half a step of fp32
+
+
+def half(dt):
+    """Half a step of a 16-bit type, relative to the value."""
+    return torch.finfo(dt).eps / 2
+
+
+def tiny(dt):
+    """Half a step among the type's subnormal numbers."""
+    return torch.finfo(dt).smallest_normal * torch.finfo(dt).eps / 2
+
+
+def codes(v):
+    """Rows in 64 bits -> (q, scale): q = rint(127 v / max|v|) with ties to even, found with whole numbers
+    (254 |v| against the odd multiples of max), so that no rounding takes part."""
+    v = v.double()
+    m = v.abs().amax(1, keepdim=True) if v.shape[1] else torch.zeros(v.shape[0], 1, dtype=torch.float64)
+    a = v.abs()
+    k = torch.floor(a * 127.0 / torch.where(m > 0, m, torch.ones_like(m)))
+    k = torch.where(k * m > 127.0 * a, k - 1, k)                  # the quotient's own rounding
+    k = torch.where((k + 1) * m <= 127.0 * a, k + 1, k)
+    up, border = 254.0 * a, (2 * k + 1) * m
+    k = k + ((up > border) | ((up == border) & (k % 2 == 1))).double()
+    k = torch.where(m > 0, k, torch.zeros_like(k))
+    return torch.sign(v) * k, (m / 127.0)[:, 0]
+
+
+def norm(x, residual, gain, eps):
+    dt = x.dtype
+    r = x.double() if residual is None else (x.double() + residual.double()).to(dt).double()
+    rstd = 1.0 / torch.sqrt(r.square().mean(1, keepdim=True) + eps)
+    p = r * gain.double()
+    q, s = codes(p)
+    return r.to(dt), p * rstd, q, s * rstd[:, 0]
+
+
+def linear(q, scale, w, w_scale, bias):
+    """(y unrounded, bound on |kernel's fp32 value - y|): the sum is exact; its conversion, the two scale
+    products and the bias's addition round once each."""
+    prod = (q.double() @ w.double().t()) * (scale.double()[:, None] * w_scale.double()[None, :])
+    y = prod if bias is None else prod + bias.double()
+    slack = 4 * U32 * prod.abs() * (1 + U32) + (0 if bias is None else 2 * U32 * (prod.abs() + bias.double().abs()))
+    return y, slack
+
+
+def assert_close16(got, want, dt, slack, what=""):
+    """got (16-bit) is want (64-bit, up to slack) rounded once."""
+    got, want = got.double().cpu(), want.cpu()
+    tol = slack + half(dt) * (want.abs() + slack) + tiny(dt)
+    bad = (got - want).abs() > tol
+    assert not bool(bad.any()), (f"{what}: {int(bad.sum())} of {bad.numel()} off, worst "
+                                 f"{float(((got - want).abs() / tol.clamp_min(1e-300)).max()):.3g} x the bound")

@@ -52,6 +52,9 @@ struct Workspace {
     int32_t *counts = nullptr, *offsets = nullptr, *perm = nullptr, *inv_perm = nullptr;
     int32_t *row_token = nullptr, *block_hist = nullptr, *err = nullptr;
     void *h = nullptr, *yp = nullptr;
+    // 8-bit activations (EK_CFG_ACT8): the call's rows and the intermediate rows as int8, one scale per row
+    uint8_t *xq = nullptr, *hq = nullptr;
+    float *xq_scale = nullptr, *hq_scale = nullptr;
     ek::WorkLists lists{};                   // device work lists (see ek_internal.h)
     int64_t list_cap[ek::kNumLists] = {0, 0, 0, 0};
     // a list of its own for a shared expert's segment cut into wide streaming items
@@ -61,7 +64,7 @@ struct Workspace {
     // launches have other shapes) and its own intermediate buffer [T, shared_inter]
     ek::WorkLists slists{};
     int64_t slist_cap[ek::kNumLists] = {0, 0, 0, 0};
-    void *hs = nullptr;
+    void *hs = nullptr;                      // ... then (EK_CFG_ACT8) the same rows as int8 and their scales
 };
 // capacities of a shared segment's own lists for at most T rows (see launch_segment_lists)
 inline int64_t shared_list_cap(int l, int64_t T)
@@ -78,6 +81,7 @@ struct ek_layer {
     bool padded = false;
     int act = 0;        // 0 bf16, 1 f16
     bool w8 = false;          // one-byte weights (int8 per channel or fp8 per block)
+    bool act8 = false;        // 8-bit activations (EK_CFG_ACT8)
     int wmode = 0;            // ek::WeightMode
     int64_t Pmax = 0;
     hipStream_t stream = nullptr;
@@ -204,7 +208,7 @@ void free_layer(ek_layer *L)
                     L->d_activation, L->st_ids, L->st_raw, L->rt_ids, L->rt_w, L->st_logits, L->st_bias, L->ws.lists.count, L->ws.lists.items[0], L->ws.lists.items[1],
                     L->ws.lists.items[2], L->ws.lists.items[3], L->ws.wide_items, L->ws.wide_count,
                     L->ws.slists.count, L->ws.slists.items[0], L->ws.slists.items[1], L->ws.slists.items[2],
-                    L->ws.slists.items[3], L->ws.hs};
+                    L->ws.slists.items[3], L->ws.hs, L->ws.xq, L->ws.hq, L->ws.xq_scale, L->ws.hq_scale};
     for (void *p : bufs) if (p) (void)hipFree(p);
     for (hipEvent_t ev : L->events) (void)hipEventDestroy(ev);
     if (L->h_err) (void)hipHostFree(L->h_err);
@@ -226,6 +230,8 @@ void free_layer(ek_layer *L)
     delete L;
 }
 
+constexpr int64_t kAct8MaxK = 131072;     // longest contraction of an int8 product
+
 ek_status validate_cfg(const ek_cfg *c)
 {
     if (!c) return fail(EK_INVALID_INPUT, "cfg is NULL");
@@ -233,7 +239,12 @@ ek_status validate_cfg(const ek_cfg *c)
         return fail(EK_INVALID_INPUT, "act_dtype must be EK_BF16 or EK_F16 (got %d)", c->act_dtype);
     if (c->w_dtype != c->act_dtype && c->w_dtype != EK_I8 && c->w_dtype != EK_F8E4M3)
         return fail(EK_INVALID_INPUT, "w_dtype must equal act_dtype or be EK_I8 or EK_F8E4M3 (got %d)", c->w_dtype);
-    if (c->flags & ~EK_CFG_BLOCK_SCALES) return fail(EK_INVALID_INPUT, "unknown flags 0x%x", c->flags);
+    if (c->flags & ~(EK_CFG_BLOCK_SCALES | EK_CFG_ACT8)) return fail(EK_INVALID_INPUT, "unknown flags 0x%x", c->flags);
+    if ((c->flags & EK_CFG_ACT8) && (c->w_dtype != EK_I8 || (c->flags & EK_CFG_BLOCK_SCALES)))
+        return fail(EK_INVALID_INPUT, "EK_CFG_ACT8 needs w_dtype EK_I8 with one scale per output channel");
+    // 127 * 127 * 131072 < 2^31: the integer sums cannot overflow
+    if ((c->flags & EK_CFG_ACT8) && (c->hidden > kAct8MaxK || c->inter > kAct8MaxK))
+        return fail(EK_INVALID_INPUT, "EK_CFG_ACT8: hidden and inter must not exceed %lld", (long long)kAct8MaxK);
     if ((c->flags & EK_CFG_BLOCK_SCALES) && c->w_dtype != EK_I8 && c->w_dtype != EK_F8E4M3)
         return fail(EK_INVALID_INPUT, "EK_CFG_BLOCK_SCALES needs w_dtype EK_I8 or EK_F8E4M3");
     if ((c->w_dtype == EK_F8E4M3 || (c->flags & EK_CFG_BLOCK_SCALES)) && (c->hidden > 8192 || c->inter > 8192))
@@ -279,6 +290,7 @@ ek_status create_layer(const ek_cfg *cfg, int64_t pmax, ek_layer **out)
     L->w8 = cfg->w_dtype == EK_I8 || cfg->w_dtype == EK_F8E4M3;
     L->wmode = cfg->w_dtype == EK_I8 ? ((cfg->flags & EK_CFG_BLOCK_SCALES) ? ek::kWI8Block : ek::kWI8)
                : cfg->w_dtype == EK_F8E4M3 ? ek::kWF8Block : ek::kW16;
+    L->act8 = (cfg->flags & EK_CFG_ACT8) != 0;
     L->Pmax = pmax;
     const int E = cfg->n_experts;
     // slot E of the tables is the shared expert; its segment (one row per token) follows the
@@ -304,6 +316,13 @@ ek_status create_layer(const ek_cfg *cfg, int64_t pmax, ek_layer **out)
     for (int i = 0; i < 10; ++i) L->forward_hist.le[i] = 4000.0 * i;   // the reference's buckets (metrics.rs:51)
     A(&L->ws.h, (size_t)rows_max * cfg->inter * 2, "h");
     A(&L->ws.yp, (size_t)rows_max * cfg->hidden * 2, "yp");
+    if (L->act8) {
+        const int64_t rows_x = std::max<int64_t>(pmax, cfg->max_tokens);
+        A((void **)&L->ws.xq, (size_t)rows_x * cfg->hidden, "8-bit rows");
+        A((void **)&L->ws.xq_scale, (size_t)rows_x * sizeof(float), "8-bit rows' scales");
+        A((void **)&L->ws.hq, (size_t)rows_max * cfg->inter, "8-bit intermediate rows");
+        A((void **)&L->ws.hq_scale, (size_t)rows_max * sizeof(float), "8-bit intermediate rows' scales");
+    }
     A((void **)&L->ws.lists.count, sizeof(int32_t) * ek::kNumLists, "work list counts");
     A((void **)&L->ws.wide_items, sizeof(ek::WorkItem) * kSharedWideItems, "shared expert's work list");
     A((void **)&L->ws.wide_count, sizeof(int32_t) * ek::kNumLists, "shared expert's work list count");
@@ -545,6 +564,12 @@ ek_status set_expert_locked(ek_layer *L, int32_t e, const ek_weight_desc *up,
     return EK_OK;
 }
 
+// Bytes of a shared expert's own intermediate rows (see Workspace::hs).
+size_t shared_rows_bytes(const ek_layer *L, int64_t T, int64_t Is)
+{
+    return (size_t)T * Is * 2 + (L->act8 ? (size_t)T * Is + (size_t)T * sizeof(float) : 0);
+}
+
 // A shared expert whose intermediate size is not the routed experts' (DeepSeek's shared_experts has
 // moe_intermediate_size * n_shared_experts channels: expertkit_torch/models/deepseek_v3/model.py:57-61):
 // its size must suit the kernels as the layer's own does, and the layer's workspace gets an
@@ -563,7 +588,9 @@ ek_status prepare_shared_width(ek_layer *L, const ek_weight_desc *up, int64_t *i
     if (ek::block_scaled(L->wmode) && Is > 8192)
         return fail(EK_INVALID_INPUT, "block-scaled layers hold at most 64 scale blocks per row: the shared expert's "
                     "intermediate size (%lld) must not exceed 8192", (long long)Is);
-    const size_t need = (size_t)L->cfg.max_tokens * Is * 2;
+    if (L->act8 && Is > kAct8MaxK)
+        return fail(EK_INVALID_INPUT, "EK_CFG_ACT8: the shared expert's intermediate size must not exceed %lld", (long long)kAct8MaxK);
+    const size_t need = shared_rows_bytes(L, L->cfg.max_tokens, Is);
     std::lock_guard<std::mutex> lk(L->mu);
     if (need > L->hs_bytes) {
         EK_HIP(hipDeviceSynchronize());
@@ -701,7 +728,13 @@ size_t carve_workspace(const ek_layer *L, int64_t T, unsigned char *base, size_t
     }
     W->h = take((size_t)rows * L->cfg.inter * 2);
     W->yp = take((size_t)rows * L->cfg.hidden * 2);
-    W->hs = L->shared_inter ? take((size_t)T * L->shared_inter * 2) : nullptr;
+    W->hs = L->shared_inter ? take(shared_rows_bytes(L, T, L->shared_inter)) : nullptr;
+    if (L->act8) {
+        W->xq = (uint8_t *)take((size_t)T * L->cfg.hidden);
+        W->xq_scale = (float *)take((size_t)T * sizeof(float));
+        W->hq = (uint8_t *)take((size_t)rows * L->cfg.inter);
+        W->hq_scale = (float *)take((size_t)rows * sizeof(float));
+    }
     return off;
 }
 
@@ -923,6 +956,43 @@ hipStream_t pick_side_stream(ek_layer *L, hipStream_t s)
     return chosen;
 }
 
+// 16-bit rows [n, K] -> int8 rows and their scales (EK_CFG_ACT8); K is a multiple of 64.
+ek_status enqueue_quant(ek_layer *L, const void *x, int64_t n, int64_t K, uint8_t *q, float *scale, hipStream_t s)
+{
+    ek::RowQuantArgs r{};
+    r.x = x; r.q = q; r.scale = scale; r.n = n; r.H = (int32_t)K; r.q_stride = (int32_t)K; r.vec = true;
+    EK_HIP(ek::launch_row_quant(r, L->act, false, s));
+    return EK_OK;
+}
+
+// enqueue_ffn on 8-bit activations: x are int8 rows with x_scale, h_rows the packed rows the lists cover.  The
+// streaming and the tile launches of a stage run in turn.
+ek_status enqueue_ffn_q8(ek_layer *L, const Workspace &W, const uint8_t *x, const float *x_scale, const int32_t *rows, void *out,
+                         int64_t h_rows, const int64_t cap[ek::kNumLists], bool wide, int64_t shared_wide, hipStream_t s, hipEvent_t *ev)
+{
+    const int64_t H = L->cfg.hidden, I = L->cfg.inter;
+    ek::Q8Args a{};
+    a.x = x; a.x_scale = x_scale; a.rows = rows; a.slabs = L->d_slabs; a.out = W.h; a.out_stride = I;
+    a.N = (int32_t)I; a.NT = (int32_t)(I / 16); a.Kdim = (int32_t)H; a.lists = W.lists;
+    const int64_t wide_cap[ek::kNumLists] = {shared_wide, 0, 0, 0};
+    for (int stage = 1; stage <= 2; ++stage) {
+        if (stage == 2) {
+            if (ev) EK_HIP(hipEventRecord(ev[2], s));
+            EK_TRY(enqueue_quant(L, W.h, h_rows, I, W.hq, W.hq_scale, s));
+            a.x = W.hq; a.x_scale = W.hq_scale; a.rows = nullptr; a.out = out; a.out_stride = H;
+            a.N = (int32_t)H; a.NT = (int32_t)(H / 16); a.Kdim = (int32_t)I;
+        }
+        EK_HIP(ek::launch_ffn_q8(a, stage, L->act, cap, wide, s));
+        if (shared_wide > 0) {
+            ek::Q8Args aw = a;               // the same stage over the shared segment's own list
+            aw.lists.items[ek::kListStream] = W.wide_items;
+            aw.lists.count = W.wide_count;
+            EK_HIP(ek::launch_ffn_q8(aw, stage, L->act, wide_cap, true, s));
+        }
+    }
+    return EK_OK;
+}
+
 // Both FFN stages over the work lists in W.lists: x [*, H] (rows picked through
 // `rows`, or packed order when nullptr) -> W.h -> out [P, H].  P and E bound the
 // list lengths (grid sizes); ev, if set, receives the stage boundary event.
@@ -935,9 +1005,11 @@ hipStream_t pick_side_stream(ek_layer *L, hipStream_t s)
 // segment); they get launches of their own on the side stream, beside the others.
 // exact: the lists' lengths when the caller built them on the host (the grids then fit them,
 // an empty list gets no launch, and the two chains run side by side exactly when both have work).
+// x_scale (EK_CFG_ACT8): x are int8 rows with these scales, the lists cover h_rows packed rows.
 ek_status enqueue_ffn(ek_layer *L, const Workspace &W, const void *x, const int32_t *rows, void *out, int64_t P, int64_t E,
                       hipStream_t s, hipEvent_t *ev, int64_t wide_items = 0, int64_t extra_stream = 0,
-                      int64_t shared_wide = 0, const int64_t *exact = nullptr, int64_t known_tile_items = -1)
+                      int64_t shared_wide = 0, const int64_t *exact = nullptr, int64_t known_tile_items = -1,
+                      const float *x_scale = nullptr, int64_t h_rows = 0)
 {
     const int64_t H = L->cfg.hidden, I = L->cfg.inter;
     ek::FfnArgs a1;
@@ -952,6 +1024,13 @@ ek_status enqueue_ffn(ek_layer *L, const Workspace &W, const void *x, const int3
         if (exact) cap[l] = exact[l];          // the caller built the lists on the host
         if (cap[l] > W.list_cap[l]) cap[l] = W.list_cap[l];
         if (cap[l] < 0) cap[l] = 0;
+    }
+    if (L->act8) {
+        if (wide_items > 0) {
+            const int64_t wcap[ek::kNumLists] = {wide_items, 0, 0, 0};
+            return enqueue_ffn_q8(L, W, (const uint8_t *)x, x_scale, rows, out, h_rows, wcap, true, 0, s, ev);
+        }
+        return enqueue_ffn_q8(L, W, (const uint8_t *)x, x_scale, rows, out, h_rows, cap, false, shared_wide, s, ev);
     }
     if (wide_items > 0) {
         EK_HIP(ek::launch_ffn_stream(a1, 1, L->act, L->wmode, wide_items, true, false, s));
@@ -1085,7 +1164,7 @@ ek_status enqueue_route(ek_layer *L, const Workspace &W, const int32_t *ids, int
 // The intermediate rows live in W.hs [T, shared_inter]: the kernels index rows by packed position,
 // so they get the address row P would have if the buffer started at row 0.
 ek_status enqueue_shared_own(ek_layer *L, const Workspace &W, const void *x, int64_t P, int64_t T, const SharedCut &sc,
-                             hipStream_t s)
+                             hipStream_t s, const float *x_scale = nullptr)
 {
     const int64_t H = L->cfg.hidden, Is = L->shared_inter;
     if (!W.hs) return fail(EK_INTERNAL, "no intermediate buffer for the shared expert");
@@ -1101,6 +1180,24 @@ ek_status enqueue_shared_own(ek_layer *L, const Workspace &W, const void *x, int
     a2.N = (int32_t)H; a2.Kdim = (int32_t)Is;
     int64_t cap[ek::kNumLists];
     for (int l = 0; l < ek::kNumLists; ++l) cap[l] = std::min<int64_t>(shared_list_cap(l, T), W.slist_cap[l]);
+    if (L->act8) {
+        uint8_t *hq = (uint8_t *)W.hs + (size_t)T * Is * 2;
+        float *hq_scale = (float *)(hq + (size_t)T * Is);
+        if (sc.streamed) { cap[ek::kListStream] = (T + 15) / 16; cap[1] = cap[2] = cap[3] = 0; }
+        else if (sc.wide) { cap[ek::kListStream] = (T + ek::kWideRows - 1) / ek::kWideRows; cap[1] = cap[2] = cap[3] = 0; }
+        else cap[ek::kListStream] = 1;
+        ek::Q8Args q{};
+        q.x = (const uint8_t *)x; q.x_scale = x_scale; q.rows = W.row_token; q.slabs = L->d_slabs; q.out = a1.out; q.out_stride = Is;
+        q.N = (int32_t)Is; q.NT = (int32_t)(Is / 16); q.Kdim = (int32_t)H; q.lists = W.slists;
+        EK_HIP(ek::launch_ffn_q8(q, 1, L->act, cap, sc.wide, side));
+        EK_TRY(enqueue_quant(L, W.hs, T, Is, hq, hq_scale, side));
+        // (rows are indexed by packed position P + t)
+        q.x = hq - (size_t)P * Is; q.x_scale = hq_scale - P; q.rows = nullptr; q.out = W.yp; q.out_stride = H;
+        q.N = (int32_t)H; q.NT = (int32_t)(H / 16); q.Kdim = (int32_t)Is;
+        EK_HIP(ek::launch_ffn_q8(q, 2, L->act, cap, sc.wide, side));
+        EK_HIP(hipEventRecord(L->ev_sjoin, side));
+        return EK_OK;
+    }
     for (int stage = 1; stage <= 2; ++stage) {
         const ek::FfnArgs &a = stage == 1 ? a1 : a2;
         if (sc.streamed) {
@@ -1134,13 +1231,15 @@ bool pair_direct_fits(const ek_layer *L, int64_t T)
 {
     const int64_t P = T * L->cfg.top_k;
     const SharedCut sc = shared_cut(L, T);          // a shared expert of the routed experts' shape is one more wave
-    return P > 0 && P <= kPairDirectPairs && L->cfg.top_k <= ek::kPairDirectMaxK && (!sc.shared || !sc.own);
+    return !L->act8 && P > 0 && P <= kPairDirectPairs && L->cfg.top_k <= ek::kPairDirectMaxK && (!sc.shared || !sc.own);
 }
 
 // want_tables: the caller reads the call's routing tables or packed expert outputs afterwards.
+// x_scale (EK_CFG_ACT8): x are int8 rows with these scales; nullptr: 16-bit rows, quantised here.
 ek_status enqueue_forward(ek_layer *L, const Workspace &W, const void *x, const int32_t *ids, const void *w, int w_f32,
                           int64_t T, void *y, hipStream_t s, bool routed = false,
-                          const std::function<ek_status()> *before_combine = nullptr, bool want_tables = true)
+                          const std::function<ek_status()> *before_combine = nullptr, bool want_tables = true,
+                          const float *x_scale = nullptr)
 {
     const int64_t H = L->cfg.hidden;
     const int E = L->cfg.n_experts, K = L->cfg.top_k;
@@ -1184,12 +1283,18 @@ ek_status enqueue_forward(ek_layer *L, const Workspace &W, const void *x, const 
     const SharedCut sc = shared_cut(L, T);
     const bool shared = sc.shared, shared_streamed = sc.streamed && !sc.own, shared_wide = sc.wide && !sc.own;
     if (ev) EK_HIP(hipEventRecord(ev[1], s));
-    if (P > 0 && sc.own) EK_TRY(enqueue_shared_own(L, W, x, P, T, sc, s));     // on the side stream, joined before the combine
+    if (L->act8 && !x_scale && P > 0) {
+        EK_TRY(enqueue_quant(L, x, T, H, W.xq, W.xq_scale, s));
+        x = W.xq;
+        x_scale = W.xq_scale;
+    }
+    if (P > 0 && sc.own) EK_TRY(enqueue_shared_own(L, W, x, P, T, sc, s, x_scale));     // on the side stream, joined before the combine
     if (P > 0) {
         const bool in_lists = shared && !shared_wide && !sc.own;   // the shared segment's items sit in the routed pairs' lists
         EK_TRY(enqueue_ffn(L, W, x, W.row_token, W.yp, in_lists ? P + T : P, in_lists ? E + 1 : E, s, ev, 0,
                            shared_streamed ? (T + 15) / 16 : 0,
-                           shared_wide ? (T + ek::kWideRows - 1) / ek::kWideRows : 0));
+                           shared_wide ? (T + ek::kWideRows - 1) / ek::kWideRows : 0, nullptr, -1,
+                           x_scale, in_lists || shared_wide ? P + T : P));
         if (sc.own) EK_HIP(hipStreamWaitEvent(s, L->ev_sjoin, 0));
         if (ev) EK_HIP(hipEventRecord(ev[3], s));
         if (before_combine) EK_TRY((*before_combine)());
@@ -1216,6 +1321,107 @@ ek_status finish_blocking(ek_layer *L, const Workspace &W, hipStream_t s)
     EK_HIP(hipStreamSynchronize(s));
     bounce_flush(L);
     return err_to_status(L->h_err[0]);
+}
+
+// Int8 rows a layer cannot read where they lie (host memory, a padded layer's row length) into its workspace:
+// *x and *scale become the workspace's.
+ek_status q8_rows_in(ek_layer *L, const void **x, const float **scale, int64_t T, int mem, hipStream_t s)
+{
+    if (T <= 0) return EK_OK;
+    const int64_t UH = L->user_hidden;
+    const void *raw = *x;
+    if (mem == EK_HOST) {
+        void *to = L->padded ? L->ws.yp : L->ws.xq;      // (yp: scratch until stage 2)
+        EK_TRY(h2d(L, to, raw, (size_t)T * UH, s));
+        EK_TRY(h2d(L, L->ws.xq_scale, *scale, (size_t)T * sizeof(float), s));
+        raw = to;
+        *scale = L->ws.xq_scale;
+    }
+    if (L->padded) EK_HIP(ek::launch_pad_rows8(raw, T, (int32_t)UH, L->ws.xq, (int32_t)L->cfg.hidden, s));
+    *x = L->padded || mem == EK_HOST ? L->ws.xq : raw;
+    return EK_OK;
+}
+
+// ek_layer_forward and (x_scale: x are int8 rows) ek_layer_forward_q8
+ek_status layer_forward(ek_layer *layer, const void *x, const float *x_scale, const int32_t *ids, const void *w, int32_t w_dtype,
+                        int64_t T, void *y, const ek_route_out *route, int32_t mem, void *stream)
+{
+    if (!layer) return fail(EK_INVALID_INPUT, "layer is NULL");
+    if (T < 0 || T > layer->cfg.max_tokens)
+        return fail(EK_INVALID_INPUT, "T = %lld outside [0, max_tokens = %lld]", (long long)T,
+                    (long long)layer->cfg.max_tokens);
+    if (mem != EK_HOST && mem != EK_DEVICE) return fail(EK_INVALID_INPUT, "bad mem %d", mem);
+    if (w_dtype != layer->cfg.act_dtype && w_dtype != EK_F32)
+        return fail(EK_INVALID_INPUT, "w_dtype must be the activation dtype or EK_F32 (got %d)",
+                    w_dtype);
+    if (T > 0 && (!x || !ids || !w || !y)) return fail(EK_INVALID_INPUT, "NULL tensor pointer");
+    if (mem == EK_HOST && stream)
+        return fail(EK_INVALID_INPUT, "host-memory calls are blocking: stream must be NULL");
+    DeviceGuard dg(layer->cfg.device_id);
+    if (!dg.ok) return fail(EK_HIP_ERROR, "hipSetDevice(%d) failed", layer->cfg.device_id);
+    Timer tm;
+    const int64_t H = layer->cfg.hidden, K = layer->cfg.top_k, P = T * K;
+    const int w_f32 = w_dtype == EK_F32;
+    std::lock_guard<std::mutex> lk(layer->mu);
+    hipStream_t s = stream ? (hipStream_t)stream : layer->stream;
+    WorkspaceUse use(layer->ev_ws, &layer->ws_busy, s);
+    EK_TRY(use.begin());
+    ek_status st = EK_OK;
+    // a blocking call on device buffers sees everything submitted before it
+    if (mem == EK_DEVICE && !stream) { EK_HIP(hipDeviceSynchronize()); use.device_idle(); }
+    if (layer->padded) {
+        EK_TRY(ensure_io_staging(layer));
+        const int32_t *d_ids = ids;
+        const void *d_w = w;
+        if (mem == EK_HOST && T > 0) {
+            EK_HIP(hipMemcpyAsync(layer->st_ids, ids, (size_t)P * 4, hipMemcpyHostToDevice, s));
+            EK_HIP(hipMemcpyAsync(layer->st_w, w, (size_t)P * (w_f32 ? 4 : 2), hipMemcpyHostToDevice, s));
+            d_ids = layer->st_ids;
+            d_w = layer->st_w;
+        }
+        const void *d_x = layer->st_x;
+        if (x_scale) {
+            EK_TRY(q8_rows_in(layer, &x, &x_scale, T, mem, s));
+            d_x = x;
+        } else {
+            EK_TRY(rows_in(layer, layer->st_x, x, T, mem, s));
+        }
+        EK_TRY(enqueue_forward(layer, layer->ws, d_x, d_ids, d_w, w_f32, T, layer->st_y, s, false, nullptr, route != nullptr, x_scale));
+        EK_TRY(rows_out(layer, y, layer->st_y, T, mem, s));
+        EK_TRY(copy_route_out(layer, layer->ws, route, P, mem, s));
+        if (!stream) { st = finish_blocking(layer, layer->ws, s); use.synced(); }
+    } else if (mem == EK_DEVICE) {
+        EK_TRY(enqueue_forward(layer, layer->ws, x, ids, w, w_f32, T, y, s, false, nullptr, route != nullptr, x_scale));
+        EK_TRY(copy_route_out(layer, layer->ws, route, P, mem, s));
+        if (!stream) { st = finish_blocking(layer, layer->ws, s); use.synced(); }
+    } else {
+        EK_TRY(ensure_io_staging(layer));
+        EK_TRY(bounce_begin(layer, s, (size_t)T * H * 2 + (size_t)P * 8));
+        if (T > 0) {
+            if (!x_scale) EK_TRY(h2d(layer, layer->st_x, x, (size_t)T * H * 2, s));
+            EK_TRY(h2d(layer, layer->st_ids, ids, (size_t)P * 4, s));
+            EK_TRY(h2d(layer, layer->st_w, w, (size_t)P * (w_f32 ? 4 : 2), s));
+        }
+        const void *d_x = layer->st_x;
+        if (x_scale) {
+            EK_TRY(q8_rows_in(layer, &x, &x_scale, T, mem, s));
+            d_x = x;
+        }
+        EK_TRY(enqueue_forward(layer, layer->ws, d_x, layer->st_ids, layer->st_w, w_f32, T,
+                               layer->st_y, s, false, nullptr, route != nullptr, x_scale));
+        if (T > 0) EK_TRY(d2h(layer, y, layer->st_y, (size_t)T * H * 2, s));
+        EK_TRY(copy_route_out(layer, layer->ws, route, P, mem, s));
+        st = finish_blocking(layer, layer->ws, s);
+        use.synced();
+    }
+    {
+        std::lock_guard<std::mutex> sl(layer->stats_mu);
+        layer->stats.forward_calls += 1;
+        layer->stats.tokens += T;
+        layer->stats.pairs += P;
+        if (!stream) { layer->stats.last_forward_us = tm.us(); observe_forward(layer, layer->stats.last_forward_us); }
+    }
+    return st;
 }
 
 }  // namespace
@@ -1321,72 +1527,19 @@ ek_status ek_layer_forward(ek_layer *layer, const void *x, const int32_t *ids, c
                            int32_t w_dtype, int64_t T, void *y, const ek_route_out *route,
                            int32_t mem, void *stream)
 {
+    EK_GUARDED(return layer_forward(layer, x, nullptr, ids, w, w_dtype, T, y, route, mem, stream);)
+}
+
+ek_status ek_layer_forward_q8(ek_layer *layer, const void *x, const float *x_scale, const int32_t *ids, const void *w,
+                              int32_t w_dtype, int64_t T, void *y, const ek_route_out *route, int32_t mem, void *stream)
+{
     EK_GUARDED(
         if (!layer) return fail(EK_INVALID_INPUT, "layer is NULL");
-        if (T < 0 || T > layer->cfg.max_tokens)
-            return fail(EK_INVALID_INPUT, "T = %lld outside [0, max_tokens = %lld]", (long long)T,
-                        (long long)layer->cfg.max_tokens);
-        if (mem != EK_HOST && mem != EK_DEVICE) return fail(EK_INVALID_INPUT, "bad mem %d", mem);
-        if (w_dtype != layer->cfg.act_dtype && w_dtype != EK_F32)
-            return fail(EK_INVALID_INPUT, "w_dtype must be the activation dtype or EK_F32 (got %d)",
-                        w_dtype);
-        if (T > 0 && (!x || !ids || !w || !y)) return fail(EK_INVALID_INPUT, "NULL tensor pointer");
-        if (mem == EK_HOST && stream)
-            return fail(EK_INVALID_INPUT, "host-memory calls are blocking: stream must be NULL");
-        DeviceGuard dg(layer->cfg.device_id);
-        if (!dg.ok) return fail(EK_HIP_ERROR, "hipSetDevice(%d) failed", layer->cfg.device_id);
-        Timer tm;
-        const int64_t H = layer->cfg.hidden, K = layer->cfg.top_k, P = T * K;
-        const int w_f32 = w_dtype == EK_F32;
-        std::lock_guard<std::mutex> lk(layer->mu);
-        hipStream_t s = stream ? (hipStream_t)stream : layer->stream;
-        WorkspaceUse use(layer->ev_ws, &layer->ws_busy, s);
-        EK_TRY(use.begin());
-        ek_status st = EK_OK;
-        // a blocking call on device buffers sees everything submitted before it
-        if (mem == EK_DEVICE && !stream) { EK_HIP(hipDeviceSynchronize()); use.device_idle(); }
-        if (layer->padded) {
-            EK_TRY(ensure_io_staging(layer));
-            const int32_t *d_ids = ids;
-            const void *d_w = w;
-            if (mem == EK_HOST && T > 0) {
-                EK_HIP(hipMemcpyAsync(layer->st_ids, ids, (size_t)P * 4, hipMemcpyHostToDevice, s));
-                EK_HIP(hipMemcpyAsync(layer->st_w, w, (size_t)P * (w_f32 ? 4 : 2), hipMemcpyHostToDevice, s));
-                d_ids = layer->st_ids;
-                d_w = layer->st_w;
-            }
-            EK_TRY(rows_in(layer, layer->st_x, x, T, mem, s));
-            EK_TRY(enqueue_forward(layer, layer->ws, layer->st_x, d_ids, d_w, w_f32, T, layer->st_y, s, false, nullptr, route != nullptr));
-            EK_TRY(rows_out(layer, y, layer->st_y, T, mem, s));
-            EK_TRY(copy_route_out(layer, layer->ws, route, P, mem, s));
-            if (!stream) { st = finish_blocking(layer, layer->ws, s); use.synced(); }
-        } else if (mem == EK_DEVICE) {
-            EK_TRY(enqueue_forward(layer, layer->ws, x, ids, w, w_f32, T, y, s, false, nullptr, route != nullptr));
-            EK_TRY(copy_route_out(layer, layer->ws, route, P, mem, s));
-            if (!stream) { st = finish_blocking(layer, layer->ws, s); use.synced(); }
-        } else {
-            EK_TRY(ensure_io_staging(layer));
-            EK_TRY(bounce_begin(layer, s, (size_t)T * H * 2 + (size_t)P * 8));
-            if (T > 0) {
-                EK_TRY(h2d(layer, layer->st_x, x, (size_t)T * H * 2, s));
-                EK_TRY(h2d(layer, layer->st_ids, ids, (size_t)P * 4, s));
-                EK_TRY(h2d(layer, layer->st_w, w, (size_t)P * (w_f32 ? 4 : 2), s));
-            }
-            EK_TRY(enqueue_forward(layer, layer->ws, layer->st_x, layer->st_ids, layer->st_w, w_f32, T,
-                                   layer->st_y, s, false, nullptr, route != nullptr));
-            if (T > 0) EK_TRY(d2h(layer, y, layer->st_y, (size_t)T * H * 2, s));
-            EK_TRY(copy_route_out(layer, layer->ws, route, P, mem, s));
-            st = finish_blocking(layer, layer->ws, s);
-            use.synced();
-        }
-        {
-            std::lock_guard<std::mutex> sl(layer->stats_mu);
-            layer->stats.forward_calls += 1;
-            layer->stats.tokens += T;
-            layer->stats.pairs += P;
-            if (!stream) { layer->stats.last_forward_us = tm.us(); observe_forward(layer, layer->stats.last_forward_us); }
-        }
-        return st;
+        if (!layer->act8) return fail(EK_INVALID_INPUT, "8-bit rows need a layer created with EK_CFG_ACT8");
+        if (T > 0 && !x_scale) return fail(EK_INVALID_INPUT, "NULL tensor pointer");
+        if (mem == EK_DEVICE && (((uintptr_t)x & 15) || ((uintptr_t)x_scale & 3)))
+            return fail(EK_INVALID_INPUT, "8-bit rows must be 16-byte aligned, their scales 4-byte aligned");
+        return layer_forward(layer, x, x_scale, ids, w, w_dtype, T, y, route, mem, stream);
     )
 }
 
@@ -1538,8 +1691,12 @@ ek_status ek_layer_expert_forward(ek_layer *layer, int32_t expert, const void *x
             const bool wide = ek::wide_cut_pays((n >> 7) + ((n & 127) > 16), n, H, layer->cfg.inter) &&
                               wide_items <= layer->ws.list_cap[ek::kListStream];
             ek::launch_single_lists(layer->ws.lists, expert, (int32_t)n, wide, s);
+            if (layer->act8) {
+                EK_TRY(enqueue_quant(layer, d_x, n, H, layer->ws.xq, layer->ws.xq_scale, s));
+                d_x = layer->ws.xq;
+            }
             EK_TRY(enqueue_ffn(layer, layer->ws, d_x, nullptr, d_out, n, 1, s, nullptr, wide ? wide_items : 0, 0, 0, nullptr,
-                               wide ? 0 : (n >> 7) + ((n & 127) > 16)));
+                               wide ? 0 : (n >> 7) + ((n & 127) > 16), layer->ws.xq_scale, n));
             if (layer->padded) EK_TRY(rows_out(layer, out, layer->st_y, n, mem, s));
             else if (mem == EK_HOST) EK_TRY(d2h(layer, out, layer->st_y, (size_t)n * H * 2, s));
         }
@@ -1746,8 +1903,13 @@ ek_status ek_layer_experts_forward(ek_layer *layer, int32_t n_calls, const int32
             }
             int64_t exact[ek::kNumLists];
             for (int l = 0; l < ek::kNumLists; ++l) exact[l] = (int64_t)items[l].size();
-            EK_TRY(enqueue_ffn(layer, layer->ws, layer->st_x, nullptr, layer->st_y, P, n_calls, s, nullptr, wide ? wide_items : 0, 0, 0,
-                               wide ? nullptr : exact));
+            const void *ffn_x = layer->st_x;
+            if (layer->act8) {
+                EK_TRY(enqueue_quant(layer, layer->st_x, P, H, layer->ws.xq, layer->ws.xq_scale, s));
+                ffn_x = layer->ws.xq;
+            }
+            EK_TRY(enqueue_ffn(layer, layer->ws, ffn_x, nullptr, layer->st_y, P, n_calls, s, nullptr, wide ? wide_items : 0, 0, 0,
+                               wide ? nullptr : exact, -1, layer->ws.xq_scale, P));
             EK_HIP(hipGetLastError());
             row0 = 0;
             if (one_transfer) {

@@ -156,14 +156,14 @@ __global__ __launch_bounds__(64 * kQ8Slices) void q8_stream_kernel(Q8Args a, int
             const float us[4] = {su.x, su.y, su.z, su.w}, gs[4] = {sg.x, sg.y, sg.z, sg.w};
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                v[r] = (float)swiglu_rounded<T>((float)tot[0][r] * (xs[rs] * us[r]), (float)tot[1][r] * (xs[rs] * gs[r]));
+                v[r] = (float)swiglu_rounded<T>(as_fp32((float)tot[0][r] * (xs[rs] * us[r])), as_fp32((float)tot[1][r] * (xs[rs] * gs[r])));
             store4<T>(orow, ch, a.N, true, v);
         } else {
             const float4 s4 = *(const float4 *)(slab.s_down + ch);
             const float ws[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                v[r] = (float)tot[0][r] * (xs[rs] * ws[r]);
+                v[r] = as_fp32((float)tot[0][r] * (xs[rs] * ws[r]));
                 if (a.bias && ch + r < a.N) v[r] += a.bias[ch + r];
             }
             store4<T>(orow, ch, a.N, (a.out_stride & 3) == 0 && ch + 4 <= a.N, v);

@@ -57,6 +57,14 @@ __device__ __forceinline__ uint4 ldg16_once(const void *p)
 
 template <typename T> __device__ __forceinline__ float rnd(float v) { return (float)(T)v; }
 
+// v, as the fp32 value it is: without this the compiler may join an fp32 product and its rounding to fp16 into one
+// instruction that rounds once (v_fma_mixlo_f16), in one kernel and not in another.
+__device__ __forceinline__ float as_fp32(float v)
+{
+    asm("" : "+v"(v));
+    return v;
+}
+
 // Two fp32 values -> one dword holding their round-to-nearest-even 16-bit forms
 // (v_cvt_pk_bf16_f32 / v_cvt_pkrtz is not used: rtz would differ from the CPU cast).
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);

@@ -85,121 +85,125 @@ template <typename T, bool NORM, int NV, int THREADS>
 __global__ __launch_bounds__(THREADS) void row_quant_kernel(RowQuantArgs a)
 {
     constexpr int WAVES = THREADS / 64;
-    const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int nvec = (a.H + 7) >> 3;
     constexpr int KEEP = NV ? NV : 1;
     float p[KEEP][8], r[NORM ? KEEP : 1][8];
-    // The squares are summed in fp64: no overflow for any finite input, and no dependence of the result on
-    // the row's length (the kernel waits for memory: the two extra instructions per element are not seen).
-    double ss = 0.0;
-    float m = 0.f;
-    auto take = [&](const float *pv, const float *rv) {
+    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+        // The squares are summed in fp64: no overflow for any finite input, and no dependence of the result on
+        // the row's length (the kernel waits for memory: the two extra instructions per element are not seen).
+        double ss = 0.0;
+        float m = 0.f;
+        auto take = [&](const float *pv, const float *rv) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if constexpr (NORM) ss = __builtin_fma((double)rv[j], (double)rv[j], ss);
-            // a NaN must not be lost: max drops it, so it is carried as an infinity
-            const float v = __builtin_fabsf(pv[j]);
-            m = v <= __builtin_huge_valf() ? __builtin_fmaxf(m, v) : __builtin_huge_valf();
-        }
-    };
-    if constexpr (NV > 0) {
-#pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int c = u * THREADS + tid;
-            if (c < nvec) {
-                row_values<T, NORM>(a, row, c * 8, p[u], NORM ? r[u] : nullptr);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) { p[u][j] = 0.f; if constexpr (NORM) r[u][j] = 0.f; }
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (NORM) ss = __builtin_fma((double)rv[j], (double)rv[j], ss);
+                // a NaN must not be lost: max drops it, so it is carried as an infinity
+                const float v = __builtin_fabsf(pv[j]);
+                m = v <= __builtin_huge_valf() ? __builtin_fmaxf(m, v) : __builtin_huge_valf();
             }
-        }
+        };
+        if constexpr (NV > 0) {
 #pragma unroll
-        for (int u = 0; u < NV; ++u) take(p[u], NORM ? r[u] : nullptr);
-    } else {
-        for (int c = tid; c < nvec; c += THREADS) {
-            row_values<T, NORM>(a, row, c * 8, p[0], r[0]);
-            take(p[0], r[0]);
-        }
-    }
+            for (int u = 0; u < NV; ++u) {
+                const int c = u * THREADS + tid;
+                if (c < nvec) {
+                    row_values<T, NORM>(a, row, c * 8, p[u], NORM ? r[u] : nullptr);
+                } else {
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        if constexpr (NORM) ss += __shfl_xor(ss, d);
-        m = __builtin_fmaxf(m, __shfl_xor(m, d));
-    }
-    if constexpr (WAVES > 1) {
-        __shared__ double s_ss[WAVES];
-        __shared__ float s_m[WAVES];
-        if (lane == 0) { s_ss[wave] = ss; s_m[wave] = m; }
-        __syncthreads();
-        ss = s_ss[0]; m = s_m[0];
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) { ss += s_ss[w]; m = __builtin_fmaxf(m, s_m[w]); }
-    }
-    float rstd = 1.f;
-    if constexpr (NORM) {
-        // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40)
-        const double ms = ss * a.inv_h + (double)a.eps;
-        const double y0 = __builtin_amdgcn_rsq(ms);
-        rstd = (float)(y0 * (1.5 - 0.5 * ms * y0 * y0));      // NaN for a row with an infinity or NaN
-    }
-    const bool finite = m < __builtin_huge_valf();
-    const float up = m < 0x1p-100f ? 0x1p64f : 1.f;
-    const float inv = m > 0.f && finite ? 127.f / (m * up) : 0.f;
-    if (a.scale && tid == 0) a.scale[row] = !finite ? __builtin_nanf("") : NORM ? m * rstd / 127.f : m / 127.f;
-
-    auto give = [&](int c, const float *pv, const float *rv) {
-        const int i = c * 8;
-        if constexpr (NORM) {
-            if (a.sum) store8<T>((T *)a.sum + row * a.H, i, rv);
-            if (a.y) {
-                float o[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = pv[j] * rstd;
-                store8<T>((T *)a.y + row * a.H, i, o);
-            }
-        }
-        if (a.q) {
-            float k[8];
-            bool all = true;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) all &= quant_fast(pv[j], inv, up, k[j]);
-            if (!all) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float t;
-                    if (!quant_fast(pv[j], inv, up, t)) k[j] = quant_exact(pv[j], m, inv, up);
+                    for (int j = 0; j < 8; ++j) { p[u][j] = 0.f; if constexpr (NORM) r[u][j] = 0.f; }
                 }
             }
-            uint32_t w[2] = {0, 0};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)(int)k[j] & 0xffu) << (8 * (j & 3));
-            if (!finite) w[0] = w[1] = 0;
-            *(uint2 *)(a.q + row * a.q_stride + i) = uint2{w[0], w[1]};
+            for (int u = 0; u < NV; ++u) take(p[u], NORM ? r[u] : nullptr);
+        } else {
+            for (int c = tid; c < nvec; c += THREADS) {
+                row_values<T, NORM>(a, row, c * 8, p[0], r[0]);
+                take(p[0], r[0]);
+            }
         }
-    };
-    if constexpr (NV > 0) {
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int c = u * THREADS + tid;
-            if (c < nvec) give(c, p[u], NORM ? r[u] : nullptr);
+        for (int d = 32; d >= 1; d >>= 1) {
+            if constexpr (NORM) ss += __shfl_xor(ss, d);
+            m = __builtin_fmaxf(m, __shfl_xor(m, d));
         }
-    } else {
-        for (int c = tid; c < nvec; c += THREADS) {
-            row_values<T, NORM>(a, row, c * 8, p[0], r[0]);
-            give(c, p[0], r[0]);
+        if constexpr (WAVES > 1) {
+            __shared__ double s_ss[WAVES];
+            __shared__ float s_m[WAVES];
+            if (lane == 0) { s_ss[wave] = ss; s_m[wave] = m; }
+            __syncthreads();
+            ss = s_ss[0]; m = s_m[0];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) { ss += s_ss[w]; m = __builtin_fmaxf(m, s_m[w]); }
         }
+        float rstd = 1.f;
+        if constexpr (NORM) {
+            // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40)
+            const double ms = ss * a.inv_h + (double)a.eps;
+            const double y0 = __builtin_amdgcn_rsq(ms);
+            rstd = (float)(y0 * (1.5 - 0.5 * ms * y0 * y0));      // NaN for a row with an infinity or NaN
+        }
+        const bool finite = m < __builtin_huge_valf();
+        const float up = m < 0x1p-100f ? 0x1p64f : 1.f;
+        const float inv = m > 0.f && finite ? 127.f / (m * up) : 0.f;
+        if (a.scale && tid == 0) a.scale[row] = !finite ? __builtin_nanf("") : NORM ? m * rstd / 127.f : m / 127.f;
+
+        auto give = [&](int c, const float *pv, const float *rv) {
+            const int i = c * 8;
+            if constexpr (NORM) {
+                if (a.sum) store8<T>((T *)a.sum + row * a.H, i, rv);
+                if (a.y) {
+                    float o[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) o[j] = as_fp32(pv[j] * rstd);
+                    store8<T>((T *)a.y + row * a.H, i, o);
+                }
+            }
+            if (a.q) {
+                float k[8];
+                bool all = true;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) all &= quant_fast(pv[j], inv, up, k[j]);
+                if (!all) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        float t;
+                        if (!quant_fast(pv[j], inv, up, t)) k[j] = quant_exact(pv[j], m, inv, up);
+                    }
+                }
+                uint32_t w[2] = {0, 0};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)(int)k[j] & 0xffu) << (8 * (j & 3));
+                if (!finite) w[0] = w[1] = 0;
+                *(uint2 *)(a.q + row * a.q_stride + i) = uint2{w[0], w[1]};
+            }
+        };
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int u = 0; u < NV; ++u) {
+                const int c = u * THREADS + tid;
+                if (c < nvec) give(c, p[u], NORM ? r[u] : nullptr);
+            }
+        } else {
+            for (int c = tid; c < nvec; c += THREADS) {
+                row_values<T, NORM>(a, row, c * 8, p[0], r[0]);
+                give(c, p[0], r[0]);
+            }
+        }
+        // the padding of an int8 row that the products read in whole steps
+        if (a.q)
+            for (int i = nvec * 8 + tid * 8; i < a.q_stride; i += THREADS * 8) *(uint2 *)(a.q + row * a.q_stride + i) = uint2{0, 0};
+        if constexpr (WAVES > 1) __syncthreads();      // the next row's sums take the same LDS
     }
-    // the padding of an int8 row that the products read in whole steps
-    if (a.q)
-        for (int i = nvec * 8 + tid * 8; i < a.q_stride; i += THREADS * 8) *(uint2 *)(a.q + row * a.q_stride + i) = uint2{0, 0};
 }
+
+constexpr int64_t kMaxRowGroups = 1 << 21;     // a launch holds less than 2^32 threads
 
 template <typename T, bool NORM>
 static void launch_rows(const RowQuantArgs &a, hipStream_t s)
 {
     const int nvec = (a.H + 7) / 8;
-    const dim3 grid((unsigned)a.n);
+    const dim3 grid((unsigned)(a.n < kMaxRowGroups ? a.n : kMaxRowGroups));
 #define EK_ROWS(NV, TH) hipLaunchKernelGGL((row_quant_kernel<T, NORM, NV, TH>), grid, dim3(TH), 0, s, a)
     if (nvec <= 64) EK_ROWS(1, 64);
     else if (nvec <= 256) EK_ROWS(1, 256);

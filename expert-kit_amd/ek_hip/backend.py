@@ -158,15 +158,17 @@ class HipLayer:
     """The experts of one MoE layer, resident in HBM, with the fused layer call."""
 
     def __init__(self, hidden: int, inter: int, n_experts: int, top_k: int, act_dtype=torch.bfloat16,
-                 w_dtype=None, max_tokens: int = 1024, device_id: int = 0, block_scales: bool = False):
+                 w_dtype=None, max_tokens: int = 1024, device_id: int = 0, block_scales: bool = False,
+                 act8: bool = False):
         """w_dtype: None (= act_dtype), torch.int8 (one scale per output channel; with block_scales the
         int8 tensors of a Block-INT8 checkpoint kept with their 128x128 scales) or torch.float8_e4m3fn
-        (an FP8 checkpoint's tensors kept with their 128x128 scales)."""
+        (an FP8 checkpoint's tensors kept with their 128x128 scales).  act8 (with torch.int8 and per-channel
+        scales): W8A8, every call multiplies 8-bit activations (EK_CFG_ACT8)."""
         self._lib = C.load()
         self.cfg = C.ek_cfg(hidden=hidden, inter=inter, n_experts=n_experts, top_k=top_k,
                             act_dtype=_DT[act_dtype], w_dtype=_DT[w_dtype or act_dtype],
                             max_tokens=max_tokens, device_id=device_id,
-                            flags=C.EK_CFG_BLOCK_SCALES if block_scales else 0)
+                            flags=(C.EK_CFG_BLOCK_SCALES if block_scales else 0) | (C.EK_CFG_ACT8 if act8 else 0))
         self.act_dtype = act_dtype
         self._h = ctypes.c_void_p()
         C.check(self._lib.ek_layer_create(ctypes.byref(self.cfg), ctypes.byref(self._h)))
@@ -222,6 +224,26 @@ class HipLayer:
         C.check(self._lib.ek_layer_forward(self._h, _ptr(x), _ptr(ids), _ptr(w), _DT[w.dtype], T, _ptr(y),
                                            ctypes.byref(ro) if ro is not None else None, _mem(x),
                                            _stream_ptr(stream)))
+        return (y, rt) if return_route else y
+
+    def forward_q8(self, q: torch.Tensor, scale: torch.Tensor, ids: torch.Tensor, w: torch.Tensor, return_route: bool = False,
+                   stream=None, out: Optional[torch.Tensor] = None):
+        """forward on rows that are 8-bit already (HipNorm's q [T,H] int8 and scale [T] fp32); needs act8."""
+        T = q.shape[0]
+        if (q.dim() != 2 or q.dtype != torch.int8 or tuple(scale.shape) != (T,) or scale.dtype != torch.float32 or ids.dim() != 2
+                or ids.dtype != torch.int32 or ids.shape[0] != T or ids.shape[1] != self.cfg.top_k or w.shape != ids.shape
+                or w.dtype not in _DT or q.shape[1] != self.cfg.hidden
+                or not q.device == scale.device == ids.device == w.device):
+            raise C.EKError(C.EK_INVALID_INPUT, "q must be [T, hidden] int8, scale [T] fp32, ids and w [T, top_k] (int32, gate weights), on one device")
+        if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != self.act_dtype or out.device != q.device or not out.is_contiguous()):
+            raise C.EKError(C.EK_INVALID_INPUT, "out must be a contiguous [T, hidden] tensor of the activation dtype beside q")
+        with (_alloc_on(stream) if out is None or return_route or not (q.is_contiguous() and scale.is_contiguous()
+                                                                      and ids.is_contiguous() and w.is_contiguous()) else _NO_CTX):
+            q, scale, ids, w = q.contiguous(), scale.contiguous(), ids.contiguous(), w.contiguous()
+            y = out if out is not None else torch.empty(q.shape, dtype=self.act_dtype, device=q.device)
+            rt, ro = self._route(T, q.device) if return_route else (None, None)
+        C.check(self._lib.ek_layer_forward_q8(self._h, _ptr(q), _ptr(scale), _ptr(ids), _ptr(w), _DT[w.dtype], T, _ptr(y),
+                                              ctypes.byref(ro) if ro is not None else None, _mem(q), _stream_ptr(stream)))
         return (y, rt) if return_route else y
 
     def forward_static(self, x: torch.Tensor, ids: torch.Tensor, w: torch.Tensor, return_route: bool = False,
@@ -454,13 +476,13 @@ class HipFFN:
 
     @classmethod
     def construct(cls, x: EKInstance, weight: ExpertWeight, act_dtype=torch.bfloat16, max_rows: int = 4096,
-                  device_id: int = 0) -> "HipFFN":
+                  device_id: int = 0, act8: bool = False) -> "HipFFN":
         lib = C.load()
         per_channel_i8 = (weight.up_w is not None and weight.up_w.dtype == torch.int8
                           and weight.up_scale is not None and weight.up_scale.dim() == 1)
         w_dtype = torch.int8 if per_channel_i8 else act_dtype
         cfg = C.ek_cfg(hidden=x.hidden, inter=x.intermediate, n_experts=1, top_k=1, act_dtype=_DT[act_dtype],
-                       w_dtype=_DT[w_dtype], max_tokens=max_rows, device_id=device_id, flags=0)
+                       w_dtype=_DT[w_dtype], max_tokens=max_rows, device_id=device_id, flags=C.EK_CFG_ACT8 if act8 else 0)
         up, k1 = _desc(weight.up_w, weight.up_scale)
         gate, k2 = _desc(weight.gate_w, weight.gate_scale)
         down, k3 = _desc(weight.down_w, weight.down_scale)

@@ -104,11 +104,17 @@ typedef struct ek_cfg {
                            dequantising at load; hidden, inter <= 8192 */
     int64_t max_tokens; /* largest T a forward call will pass */
     int32_t device_id;  /* HIP device ordinal */
-    int32_t flags;      /* 0, or EK_CFG_BLOCK_SCALES */
+    int32_t flags;      /* 0, EK_CFG_BLOCK_SCALES or EK_CFG_ACT8 */
 } ek_cfg;
 /* With w_dtype EK_I8: the weights are the int8 tensors of a Block-INT8 checkpoint, kept with
  * their 128x128 block scales like the fp8 form (EK_F8E4M3 implies it). */
 #define EK_CFG_BLOCK_SCALES 1
+/* With w_dtype EK_I8 and per-channel scales: W8A8.  Every entry point of the layer multiplies 8-bit
+ * activations: a call's 16-bit rows are quantised row by row (see "8-bit activations" below),
+ * up and gate are int8 products, each rounded to act_dtype once, h = up * silu(gate) has the layer's
+ * usual storage roundings and is quantised row by row again for the down product.
+ * hidden, inter <= 131072. */
+#define EK_CFG_ACT8 2
 
 /* One weight matrix of ExpertWeight<T> (ek-computation/src/ffn/meta.rs:10-23),
  * row-major [rows = out_features, cols = in_features] as HF nn.Linear stores
@@ -222,6 +228,12 @@ ek_status ek_layer_has_expert(ek_layer *layer, int32_t expert, int32_t *loaded);
 ek_status ek_layer_forward(ek_layer *layer, const void *x, const int32_t *ids, const void *w,
                            int32_t w_dtype, int64_t T, void *y, const ek_route_out *route,
                            int32_t mem, void *stream);
+
+/* ek_layer_forward on rows that are 8-bit already (ek_norm_forward's q and scale): x [T, hidden] int8,
+ * x_scale [T] fp32.  The layer was created with EK_CFG_ACT8; everything else as in ek_layer_forward, and
+ * the same bits as its call on 16-bit rows whose quantisation is (x, x_scale). */
+ek_status ek_layer_forward_q8(ek_layer *layer, const void *x, const float *x_scale, const int32_t *ids, const void *w,
+                              int32_t w_dtype, int64_t T, void *y, const ek_route_out *route, int32_t mem, void *stream);
 
 /* ek_layer_forward for callers that cannot allocate device memory: code under HIP graph
  * capture, tight serving loops, harnesses that forbid hipMalloc.  It has no counterpart in

@@ -55,3 +55,58 @@ def assert_close16(got, want, dt, slack, what=""):
     bad = (got - want).abs() > tol
     assert not bool(bad.any()), (f"{what}: {int(bad.sum())} of {bad.numel()} off, worst "
                                  f"{float(((got - want).abs() / tol.clamp_min(1e-300)).max()):.3g} x the bound")
+
+
+# ---- the layer, in the kernels' own fp32 operations (bit for bit) -------------------------------------
+
+def _fma(a, b, c):
+    """fp32 fused multiply-add: the product of two fp32 values is exact in fp64."""
+    return (a.double() * b.double() + c.double()).float()
+
+
+def expf(x):
+    """The kernels' exp from IEEE operations (Cody-Waite reduction by ln 2, Cephes' degree-5 polynomial)."""
+    f = lambda v: torch.tensor(v, dtype=torch.float32)
+    x = x.clamp(-87.0, 89.0)
+    n = torch.round(x * f(1.44269504088896341))
+    r = _fma(n, f(-0.693359375), x)
+    r = _fma(n, f(2.12194440e-4), r)
+    p = f(1.9875691500e-4).expand_as(r)
+    for c in (1.3981999507e-3, 8.3334519073e-3, 4.1665795894e-2, 1.6666665459e-1, 5.0000001201e-1):
+        p = _fma(p, r, f(c).expand_as(r))
+    y = _fma(r * r, p, r) + 1.0
+    return (y.double() * torch.exp2(n.double())).float()
+
+
+def product(q, scale, w, w_scale):
+    """fp32(sum) * (scale * w_scale): the sum is exact, each operation rounds to fp32."""
+    acc = (q.double() @ w.double().t()).to(torch.int32).float()
+    return acc * (scale.float()[:, None] * w_scale.float()[None, :])
+
+
+def quantise(x16):
+    q, s = codes(x16)
+    return q, (x16.float().abs().amax(1) / 127.0)
+
+
+def expert(q, scale, ew, dt):
+    """8-bit rows through one expert (ek_hip.ExpertWeight) -> 16-bit rows."""
+    u = product(q, scale, ew.up_w, ew.up_scale).to(dt).float()
+    g = product(q, scale, ew.gate_w, ew.gate_scale).to(dt).float()
+    h = (u * (g / (1.0 + expf(-g))).to(dt).float()).to(dt)
+    hq, hs = quantise(h)
+    return product(hq, hs, ew.down_w, ew.down_scale).to(dt)
+
+
+def layer(q, scale, ids, w, experts, dt, shared=None):
+    T, K = ids.shape
+    out = torch.zeros(T, K, q.shape[1], dtype=dt)
+    for e in torch.unique(ids).tolist():
+        t, k = (ids == e).nonzero(as_tuple=True)
+        out[t, k] = expert(q[t], scale[t], experts[e], dt)
+    acc = torch.zeros(T, q.shape[1])
+    for k in range(K):
+        p = w[:, k].float()[:, None] * out[:, k].float()
+        acc = acc + (p if w.dtype == torch.float32 else p.to(dt).float())
+    y = acc.to(dt)
+    return y if shared is None else (y.float() + expert(q, scale, shared, dt).float()).to(dt)

@@ -327,6 +327,7 @@ ek_status create_layer(const ek_cfg *cfg, int64_t pmax, ek_layer **out)
     A((void **)&L->ws.wide_items, sizeof(ek::WorkItem) * kSharedWideItems, "shared expert's work list");
     A((void **)&L->ws.wide_count, sizeof(int32_t) * ek::kNumLists, "shared expert's work list count");
     A((void **)&L->ws.slists.count, sizeof(int32_t) * ek::kNumLists, "shared expert's work list counts");
+    L->ws.lists.one_class = L->ws.slists.one_class = L->act8;
     for (int l = 0; l < ek::kNumLists; ++l) {
         L->ws.slist_cap[l] = shared_list_cap(l, cfg->max_tokens);
         A((void **)&L->ws.slists.items[l], sizeof(ek::WorkItem) * L->ws.slist_cap[l], "shared expert's work list");
@@ -341,7 +342,8 @@ ek_status create_layer(const ek_cfg *cfg, int64_t pmax, ek_layer **out)
         const int64_t min_rows[ek::kNumLists] = {1, 17, 33, 65};
         int64_t cap = rows_max / min_rows[l] + (l == ek::kListStream ? 264 : 1);
         if (l == ek::kListStream && cap > 65535) cap = 65535;
-        if (cap < ek::list_capacity(l, rows_max, E + 1) + 1) cap = ek::list_capacity(l, rows_max, E + 1) + 1;
+        if (L->act8 && l == ek::kListT128) cap = rows_max / 17 + 1;     // every segment's remainder joins this list
+        if (cap < ek::list_capacity(l, rows_max, E + 1, L->act8) + 1) cap = ek::list_capacity(l, rows_max, E + 1, L->act8) + 1;
         L->ws.list_cap[l] = cap;
         A((void **)&L->ws.lists.items[l], sizeof(ek::WorkItem) * cap, "work list");
     }
@@ -718,9 +720,10 @@ size_t carve_workspace(const ek_layer *L, int64_t T, unsigned char *base, size_t
     W->wide_items = (ek::WorkItem *)take(sizeof(ek::WorkItem) * kSharedWideItems);
     W->wide_count = (int32_t *)take(sizeof(int32_t) * ek::kNumLists);
     for (int l = 0; l < ek::kNumLists; ++l) {
-        W->list_cap[l] = ek::list_capacity(l, rows, E + 1) + (l == ek::kListStream ? 264 : 1);
+        W->list_cap[l] = ek::list_capacity(l, rows, E + 1, L->act8) + (l == ek::kListStream ? 264 : 1);
         W->lists.items[l] = (ek::WorkItem *)take(sizeof(ek::WorkItem) * (size_t)W->list_cap[l]);
     }
+    W->lists.one_class = W->slists.one_class = L->act8;
     W->slists.count = (int32_t *)take(sizeof(int32_t) * ek::kNumLists);
     for (int l = 0; l < ek::kNumLists; ++l) {
         W->slist_cap[l] = shared_list_cap(l, T);
@@ -1020,7 +1023,7 @@ ek_status enqueue_ffn(ek_layer *L, const Workspace &W, const void *x, const int3
     a2.N = (int32_t)H; a2.Kdim = (int32_t)I;
     int64_t cap[ek::kNumLists];
     for (int l = 0; l < ek::kNumLists; ++l) {
-        cap[l] = ek::list_capacity(l, P, E) + (l == ek::kListStream ? extra_stream : 0);
+        cap[l] = ek::list_capacity(l, P, E, L->act8) + (l == ek::kListStream ? extra_stream : 0);
         if (exact) cap[l] = exact[l];          // the caller built the lists on the host
         if (cap[l] > W.list_cap[l]) cap[l] = W.list_cap[l];
         if (cap[l] < 0) cap[l] = 0;
@@ -1794,7 +1797,7 @@ ek_status ek_layer_experts_forward(ek_layer *layer, int32_t n_calls, const int32
                 for (int32_t t = 0; t < full; ++t)
                     items[ek::kListT128].push_back(ek::WorkItem{experts[i], (int32_t)row0 + t * 128, 128, 0});
                 const ek::WorkItem rem{experts[i], (int32_t)row0 + full * 128, r, 0};
-                if (r > 64) items[ek::kListT128].push_back(rem);
+                if (r > 64 || (layer->act8 && n > 16 && r > 0)) items[ek::kListT128].push_back(rem);
                 else if (r > 32) items[ek::kListT64].push_back(rem);
                 else if (r > 16) items[ek::kListT32].push_back(rem);
                 else if (r > 0) items[ek::kListStream].push_back(rem);

@@ -10,6 +10,8 @@
 #include "ek_internal.h"
 #include "ek_mfma.h"
 
+#include <type_traits>
+
 namespace ek {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
@@ -171,21 +173,275 @@ __global__ __launch_bounds__(64 * kQ8Slices) void q8_stream_kernel(Q8Args a, int
     }
 }
 
+
+// ---- tile kernel: items of up to 128 rows -------------------------------------------------------------
+//
+// One workgroup of four wavefronts: RB*32 rows x 4*64 matrix channels (stage 1: 128 hidden channels, up and
+// gate of each); every wave keeps all the rows and 64 channels.  MFMA 32x32x32 i8, weights as the A
+// operand.  Steps of 128 contraction elements:
+//   - weights go from memory straight into registers, no other wave wants them: a 16-byte load per lane
+//     from the chunked layout is an A operand, loaded one step ahead into the registers its predecessor has
+//     just left;
+//   - the rows' bytes are shared by the four waves: LDS-DMA into three stages (two steps ahead), rows of 128
+//     bytes whose 16-byte pieces are XOR-swizzled so that fragment reads are conflict free.
+// Per step and workgroup the LDS takes 16 KiB and gives 64 KiB against 1024 cycles of MFMA (128 rows): half
+// its bandwidth.  Two workgroups fit a CU (registers: 256 per lane), so that one's epilogue and first loads
+// hide behind the other's products.
+typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ void dma16(const void *gaddr, uint32_t lds_addr)     // lane l's 16 bytes land at lds_addr + 16 l
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(gaddr), "s"(lds_addr) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+// The wave has its LDS reads back before it lets the others overwrite what it read.
+__device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+
+constexpr int kQ8Waves = 4, kQ8Stages = 3;
+constexpr int kQ8Stage = 128 * 128;                       // bytes of a stage: 128 rows x 128 elements
+constexpr int kQ8ScratchPitch = 64 * 2 + 16;              // epilogue: 32 rows x 64 channels of a wave
+constexpr int kQ8Scratch = 32 * kQ8ScratchPitch;
+constexpr int kQ8Lds = kQ8Stages * kQ8Stage + kQ8Waves * kQ8Scratch;
+
+__device__ __forceinline__ int q8_key(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+
+template <typename T, int NMAT, int RB>
+__device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab, int row0, int n, int cblock, uint8_t *lds)
+{
+    const uint8_t *wmat = NMAT == 2 ? slab.upgate : slab.down;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, kh = lane >> 5, j = lane & 15;
+    const int KT = a.Kdim >> 6, nfull = KT >> 1, ns = (KT + 1) >> 1;
+    const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    // the wave's first 16-channel tile; block cb: matrix cb of tiles nt0, nt0 + 1, or tiles nt0 + 2 cb, + 1
+    const int nt0 = (cblock * kQ8Waves + wave) * (NMAT == 2 ? 2 : 4);
+    const uint8_t *wp[2];
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+        const int nt = min(nt0 + (NMAT == 2 ? 0 : cb * 2) + (l32 >> 4), a.NT - 1);   // tiles past the last recompute it
+        wp[cb] = wmat + ((int64_t)nt * KT * NMAT + (NMAT == 2 ? cb : 0)) * kChunkBytes + (kh * 16 + j) * 16;
+    }
+    // rows: DMA instruction q brings rows 8q .. 8q+7, lane l piece (l & 7) ^ key of row 8q + l / 8
+    const uint8_t *xsrc[RB];
+    int32_t tail_fix[RB];            // half a step at the end: lanes of its upper half re-read the lower one
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+        const int r = (wave * RB + i) * 8 + (lane >> 3);
+        const int rr = min(r, n - 1);                            // rows past the item re-read its last one
+        const int64_t row = a.rows ? (int64_t)a.rows[row0 + rr] : (int64_t)(row0 + rr);
+        const int piece = (lane & 7) ^ q8_key(r);
+        xsrc[i] = a.x + row * a.Kdim + piece * 16;
+        tail_fix[i] = (piece & 4) ? 64 : 0;
+    }
+    float xs[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int rr = min(rb * 32 + l32, n - 1);
+        xs[rb] = a.x_scale[a.rows ? (int64_t)a.rows[row0 + rr] : (int64_t)(row0 + rr)];
+    }
+    const int bkey = q8_key(l32);
+    int boff[4];
+#pragma unroll
+    for (int kg = 0; kg < 4; ++kg) boff[kg] = l32 * 128 + ((kg * 2 + kh) ^ bkey) * 16;
+
+    i32x16 acc[RB][2];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[rb][cb][r] = 0;
+
+    // DMAs of step s into its stage (steps past the last one repeat it: in bounds, into a stage that is free)
+    auto issue = [&](int s, int stage) {
+        const int sc = min(s, ns - 1);
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+            dma16(xsrc[i] + (int64_t)sc * 128 - (sc == nfull ? tail_fix[i] : 0), lds_base + stage * kQ8Stage + (wave * RB + i) * 1024);
+    };
+    uint4 w[4][2];
+    // one k-group's weights of the step wp points to; hi: from there to the step's second chunk
+    auto load_w = [&](int kg, int hi) {
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) w[kg][cb] = ldg16(wp[cb] + (kg >= 2 ? hi : 0) + (kg & 1) * 512);
+    };
+    // KGS k-groups of a step; REFILL: their weight registers are loaded again, for the step wp points to.  The
+    // fences keep the compiler from gathering the loads at the end of the step, and from converting all
+    // weights at its start (which would wait for the last of them).
+    auto body = [&](int stage, int hi, auto kgs_c, auto refill_c) {
+        constexpr int KGS = decltype(kgs_c)::value;
+        constexpr bool REFILL = decltype(refill_c)::value;
+        const uint8_t *st = lds + stage * kQ8Stage;
+        i32x4 b[2][RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) b[0][rb] = *(const i32x4 *)(st + boff[0] + rb * 4096);
+#pragma unroll
+        for (int kg = 0; kg < KGS; ++kg) {
+            if (kg + 1 < KGS) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) b[(kg + 1) & 1][rb] = *(const i32x4 *)(st + boff[kg + 1] + rb * 4096);
+            }
+#pragma unroll
+            for (int cb = 0; cb < 2; ++cb) {
+                const i32x4 q = signed8(w[kg][cb]);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+                    acc[rb][cb] = __builtin_amdgcn_mfma_i32_32x32x32_i8(q, b[kg & 1][rb], acc[rb][cb], 0, 0, 0);
+            }
+            if (REFILL) load_w(kg, hi);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    issue(0, 0);
+    issue(1, 1);
+#pragma unroll
+    for (int kg = 0; kg < 4; ++kg) load_w(kg, NMAT * kChunkBytes);           // (K >= 128: the first step is whole)
+
+    // At the start of step s this wave's DMAs of the step have landed when no more than the loads younger than them are
+    // outstanding: the DMAs of step s + 1 and one step's weights.  Every step issues the same number of loads; those for
+    // steps past the last one repeat what is there (half a step at the end: its one chunk twice).
+    int stage = 0, s = 0;
+    auto open = [&] {
+        wait_vmcnt<RB + 8>();
+        block_barrier();              // everyone's rows are there, and the stage of step s - 1 is free
+        issue(s + 2, stage == 0 ? 2 : stage - 1);
+    };
+    for (; s < nfull; ++s) {
+        open();
+        const int adv = s + 1 < ns ? 2 * NMAT * kChunkBytes : 0;
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb) wp[cb] += adv;
+        body(stage, s + 1 == nfull && nfull < ns ? 0 : NMAT * kChunkBytes, std::integral_constant<int, 4>{}, std::true_type{});
+        stage = stage == 2 ? 0 : stage + 1;
+    }
+    if (nfull < ns) {
+        open();
+        body(stage, 0, std::integral_constant<int, 2>{}, std::false_type{});
+    }
+    wait_vmcnt<0>();                  // the repeated loads
+
+    // Epilogue.  Register 4 q + r of a lane: channel 8 q + 4 kh + r of its block, row l32 of row block rb.  The values
+    // become 16-bit rows in the wave's scratch and leave in 16-byte pieces.
+    uint8_t *scratch = lds + kQ8Stages * kQ8Stage + wave * kQ8Scratch;
+    constexpr int NC = NMAT == 2 ? 32 : 64;                      // output channels of the wave
+    const int c0 = nt0 * 16;
+    const int nch = min(a.N - c0, NC);
+    constexpr int PPR = NC / 8;                                  // 16-byte pieces per row
+    const bool whole = nch == NC && (a.out_stride & 7) == 0;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    float ws[2][16];
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int nt = min(nt0 + (NMAT == 2 ? 0 : cb * 2) + (q >> 1), a.NT - 1);
+            const float *sp = (NMAT == 2 ? (cb == 0 ? slab.s_up : slab.s_gate) : slab.s_down) + nt * 16 + (q & 1) * 8 + kh * 4;
+            const float4 v = *(const float4 *)sp;
+            ws[cb][q * 4] = v.x; ws[cb][q * 4 + 1] = v.y; ws[cb][q * 4 + 2] = v.z; ws[cb][q * 4 + 3] = v.w;
+        }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        if (rb * 32 >= n) break;
+#pragma unroll
+        for (int cb = 0; cb < (NMAT == 2 ? 1 : 2); ++cb)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                T4 o;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = q * 4 + r;
+                    if constexpr (NMAT == 2) {
+                        o[r] = swiglu_rounded<T>(as_fp32((float)acc[rb][0][i] * (xs[rb] * ws[0][i])),
+                                                 as_fp32((float)acc[rb][1][i] * (xs[rb] * ws[1][i])));
+                    } else {
+                        float v = as_fp32((float)acc[rb][cb][i] * (xs[rb] * ws[cb][i]));
+                        const int ch = c0 + cb * 32 + q * 8 + kh * 4 + r;
+                        if (a.bias && ch < a.N) v += a.bias[ch];
+                        o[r] = (T)v;
+                    }
+                }
+                *(T4 *)(scratch + l32 * kQ8ScratchPitch + (cb * 32 + q * 8 + kh * 4) * 2) = o;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 32 * PPR / 64; ++i) {
+            const int r = (i * 64 + lane) / PPR, c = (lane % PPR) * 8;
+            if (rb * 32 + r >= n) continue;
+            T *orow = (T *)a.out + (int64_t)(row0 + rb * 32 + r) * a.out_stride + c0;
+            const uint8_t *src = scratch + r * kQ8ScratchPitch + c * 2;
+            if (whole) {
+                *(uint4 *)(orow + c) = *(const uint4 *)src;
+            } else {
+                for (int k = 0; k < 8; ++k)
+                    if (c + k < nch) orow[c + k] = ((const T *)src)[k];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+// Tiles are numbered item by item; XCD x (workgroups x, x + 8, ...) walks a contiguous eighth of them, so that
+// the workgroups that share an item's rows or an expert's weights share an L2.
+template <typename T, int NMAT>
+__global__ __launch_bounds__(64 * kQ8Waves, 2) void q8_tile_kernel(Q8Args a, int cblocks)
+{
+    extern __shared__ __align__(1024) uint8_t q8_lds[];
+    const int items = a.dense_rows > 0 ? (int)((a.dense_rows + 127) >> 7) : a.lists.count[kListT128];
+    const int64_t tiles = (int64_t)items * cblocks;
+    const int64_t per = (tiles + 7) >> 3, at = blockIdx.x >> 3;
+    const int64_t tile = (int64_t)(blockIdx.x & 7) * per + at;
+    if (at >= per || tile >= tiles) return;
+    const int it = (int)(tile / cblocks), cblock = (int)(tile - (int64_t)it * cblocks);
+    int e = 0, row0, n;
+    if (a.dense_rows > 0) {
+        row0 = it * 128;
+        n = (int)min((int64_t)128, a.dense_rows - row0);
+    } else {
+        const WorkItem item = a.lists.items[kListT128][it];
+        e = item.expert; row0 = item.row0; n = item.nrows;
+    }
+    e = __builtin_amdgcn_readfirstlane(e);
+    row0 = __builtin_amdgcn_readfirstlane(row0);
+    n = __builtin_amdgcn_readfirstlane(n);
+    const ExpertSlab slab = a.slabs[e];
+    if ((NMAT == 2 ? slab.upgate : slab.down) == nullptr) return;          // expert not loaded: the call has been flagged
+    switch ((n + 31) >> 5) {
+    case 1: q8_tile<T, NMAT, 1>(a, slab, row0, n, cblock, q8_lds); break;
+    case 2: q8_tile<T, NMAT, 2>(a, slab, row0, n, cblock, q8_lds); break;
+    case 3: q8_tile<T, NMAT, 3>(a, slab, row0, n, cblock, q8_lds); break;
+    default: q8_tile<T, NMAT, 4>(a, slab, row0, n, cblock, q8_lds); break;
+    }
+}
+
+template <typename T, int NMAT>
+static hipError_t launch_tiles(const Q8Args &a, int64_t max_items, hipStream_t s)
+{
+    const int per = NMAT == 2 ? 2 * kQ8Waves : 4 * kQ8Waves;    // 16-channel tiles per workgroup
+    const int cblocks = (a.NT + per - 1) / per;
+    const int64_t tiles = max_items * cblocks, grid = (tiles + 7) / 8 * 8;
+    if (grid > (int64_t)1 << 23) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((q8_tile_kernel<T, NMAT>), dim3((unsigned)grid), dim3(64 * kQ8Waves), kQ8Lds, s, a, cblocks);
+    return hipGetLastError();
+}
+
 template <typename T, int NMAT>
 static hipError_t launch_lists(const Q8Args &a, const int64_t max_items[kNumLists], bool wide, hipStream_t s)
 {
     const dim3 block(64 * kQ8Slices);
-    auto grid = [&](int64_t items, int parts) { return dim3((unsigned)a.NT, (unsigned)items, (unsigned)parts); };
     if (max_items[kListStream] > 0) {
-        if (wide) hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 4, 2>), grid(max_items[kListStream], 1), block, 0, s, a, kListStream, 0);
-        else hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 1, 2>), grid(max_items[kListStream], 1), block, 0, s, a, kListStream, 0);
+        const dim3 grid((unsigned)a.NT, (unsigned)max_items[kListStream]);
+        if (wide) hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 4, 2>), grid, block, 0, s, a, kListStream, 0);
+        else hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 1, 2>), grid, block, 0, s, a, kListStream, 0);
     }
-    if (max_items[kListT32] > 0)
-        hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 2, 2>), grid(max_items[kListT32], 1), block, 0, s, a, kListT32, 0);
-    if (max_items[kListT64] > 0)
-        hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 4, 2>), grid(max_items[kListT64], 1), block, 0, s, a, kListT64, 0);
-    if (max_items[kListT128] > 0)
-        hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 4, 2>), grid(max_items[kListT128], 2), block, 0, s, a, kListT128, 0);
+    if (max_items[kListT128] > 0) {
+        const hipError_t e = launch_tiles<T, NMAT>(a, max_items[kListT128], s);
+        if (e != hipSuccess) return e;
+    }
     return hipGetLastError();
 }
 
@@ -201,7 +457,8 @@ template <typename T> static hipError_t launch_dense_t(const Q8Args &a, hipStrea
     const int64_t n = a.dense_rows;
     const dim3 block(64 * kQ8Slices);
     if (n <= 16) hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 1, 2>), dim3((unsigned)a.NT, 1), block, 0, s, a, 0, 16);
-    else hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 4, 2>), dim3((unsigned)a.NT, (unsigned)((n + 63) / 64)), block, 0, s, a, 0, 64);
+    else if (n <= 128) hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 4, 2>), dim3((unsigned)a.NT, (unsigned)((n + 63) / 64)), block, 0, s, a, 0, 64);
+    else return launch_tiles<T, 1>(a, (n + 127) / 128, s);
     return hipGetLastError();
 }
 

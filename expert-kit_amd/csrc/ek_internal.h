@@ -59,6 +59,9 @@ enum { kListStream = 0, kListT32 = 1, kListT64 = 2, kListT128 = 3, kNumLists = 4
 struct WorkLists {
     WorkItem *items[kNumLists];
     int32_t *count;              // [kNumLists]
+    // 1: a segment of more than 16 rows goes into the 128-row list whole, its remainder of any length included
+    // (layers on 8-bit activations, whose tile kernel takes items of 1 .. 128 rows)
+    int32_t one_class = 0;
 };
 constexpr int kWideRows = 64;
 // tile_items: work items the ordinary cut would give the tile kernel; one of them spreads
@@ -78,8 +81,9 @@ inline bool wide_cut_pays(int64_t tile_items, int64_t rows, int64_t hidden, int6
     const double streamed_us = (double)rows * (0.053 + 1.48e-8 * (double)hidden * (double)inter);
     return streamed_us < 0.92 * tile_call_us(hidden, inter);
 }
-inline int64_t list_capacity(int list, int64_t P, int64_t E)
+inline int64_t list_capacity(int list, int64_t P, int64_t E, bool one_class = false)
 {
+    if (one_class && list != kListStream) return list == kListT128 ? P / 128 + (P / 17 < E ? P / 17 : E) : 0;
     const int64_t min_rows[kNumLists] = {1, 17, 33, 65};
     const int64_t by_rows = P / min_rows[list];
     if (list == kListT128) return by_rows;

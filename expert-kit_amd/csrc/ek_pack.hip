@@ -100,9 +100,15 @@ __device__ __forceinline__ void block_exclusive_scan5(const int32_t (&v)[5], int
 struct SegmentCut {
     int32_t n128, n64, n32, ns;
 };
-__device__ __forceinline__ SegmentCut cut_segment(int32_t n)
+__device__ __forceinline__ SegmentCut cut_segment(int32_t n, int32_t one_class)
 {
     SegmentCut c;
+    if (one_class) {
+        c.n128 = n > 16 ? (n + 127) >> 7 : 0;
+        c.n64 = c.n32 = 0;
+        c.ns = n > 0 && n <= 16;
+        return c;
+    }
     const int32_t r = n & 127;
     c.n128 = (n >> 7) + (r > 64);
     c.n64 = r > 32 && r <= 64;
@@ -110,13 +116,14 @@ __device__ __forceinline__ SegmentCut cut_segment(int32_t n)
     c.ns = r > 0 && r <= 16;
     return c;
 }
+// items of rows seg0 .. seg0+n-1, which end a segment of seg_n rows
 __device__ __forceinline__ void emit_items(const WorkLists &l, int32_t e, int32_t seg0, int32_t n,
-                                           int32_t p128, int32_t p64, int32_t p32, int32_t ps)
+                                           int32_t p128, int32_t p64, int32_t p32, int32_t ps, int32_t seg_n)
 {
     const int32_t full = n >> 7, r = n & 127;
     for (int32_t t = 0; t < full; ++t) l.items[kListT128][p128 + t] = WorkItem{e, seg0 + t * 128, 128, 0};
     const WorkItem rem{e, seg0 + full * 128, r, 0};
-    if (r > 64) l.items[kListT128][p128 + full] = rem;
+    if (r > 64 || (l.one_class && seg_n > 16 && r > 0)) l.items[kListT128][p128 + full] = rem;
     else if (r > 32) l.items[kListT64][p64] = rem;
     else if (r > 16) l.items[kListT32][p32] = rem;
     else if (r > 0) l.items[kListStream][ps] = rem;
@@ -156,13 +163,13 @@ __global__ __launch_bounds__(1024) void pack_scan_kernel(PackArgs a)
         a.err[0] = ((int64_t)sum != a.P ? 1 : 0) | (any_unloaded ? 2 : 0);
     }
     if (a.lists.count == nullptr) return;
-    const SegmentCut c = cut_segment(total);
+    const SegmentCut c = cut_segment(total, a.lists.one_class);
     int32_t s128, s64, s32, ss;
     const int32_t p128 = block_exclusive_scan(c.n128, wave_tot, &s128);
     const int32_t p64 = block_exclusive_scan(c.n64, wave_tot, &s64);
     const int32_t p32 = block_exclusive_scan(c.n32, wave_tot, &s32);
     const int32_t ps = block_exclusive_scan(c.ns, wave_tot, &ss);
-    if (e < a.E && total > 0) emit_items(a.lists, e, off, total, p128, p64, p32, ps);
+    if (e < a.E && total > 0) emit_items(a.lists, e, off, total, p128, p64, p32, ps, total);
     if (e == 0) {
         a.lists.count[kListT128] = s128;
         a.lists.count[kListT64] = s64;
@@ -190,11 +197,11 @@ __global__ __launch_bounds__(256) void segment_lists_kernel(WorkLists l, int32_t
         }
         return;
     }
-    const SegmentCut c = cut_segment(n);
+    const SegmentCut c = cut_segment(n, l.one_class);
     const int32_t full = n >> 7;
     for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][t] = WorkItem{e, row0 + t * 128, 128, 0};
     if (threadIdx.x == 0) {
-        if (n & 127) emit_items(l, e, row0 + full * 128, n & 127, full, 0, 0, 0);    // the remainder, into its class
+        if (n & 127) emit_items(l, e, row0 + full * 128, n & 127, full, 0, 0, 0, n);    // the remainder, into its class
         l.count[kListT128] = c.n128;
         l.count[kListT64] = c.n64;
         l.count[kListT32] = c.n32;
@@ -221,16 +228,12 @@ __global__ __launch_bounds__(256) void append_segment_kernel(WorkLists l, int32_
         if (threadIdx.x == 0) l.count[kListStream] = at + items;
         return;
     }
-    const SegmentCut c = cut_segment(n);
+    const SegmentCut c = cut_segment(n, l.one_class);
     const int32_t full = n >> 7, r = n & 127;
     for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][p128 + t] = WorkItem{e, row0 + t * 128, 128, 0};
     for (int32_t t = threadIdx.x; t < n; t += 256) row_token[row0 + t] = t;
     if (threadIdx.x == 0) {
-        const WorkItem rem{e, row0 + full * 128, r, 0};
-        if (r > 64) l.items[kListT128][p128 + full] = rem;
-        else if (r > 32) l.items[kListT64][p64] = rem;
-        else if (r > 16) l.items[kListT32][p32] = rem;
-        else if (r > 0) l.items[kListStream][ps] = rem;
+        if (r > 0) emit_items(l, e, row0 + full * 128, r, p128 + full, p64, p32, ps, n);
         l.count[kListT128] = p128 + c.n128;
         l.count[kListT64] = p64 + c.n64;
         l.count[kListT32] = p32 + c.n32;
@@ -350,7 +353,7 @@ __global__ __launch_bounds__(1024) void pack_fused_kernel(PackArgs a, int nbits)
         if (total > 0 && a.slabs != nullptr && a.slabs[e].upgate == nullptr) atomicOr(lerr, 2);
     }
     // offsets and the four lists' positions in one scan
-    const SegmentCut c = cut_segment(total);
+    const SegmentCut c = cut_segment(total, a.lists.one_class);
     const int32_t v5[5] = {total, c.n128, c.n64, c.n32, c.ns};
     int32_t ex[5], tot5[5];
     block_exclusive_scan5(v5, wave_tot5, ex, tot5);
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(1024) void pack_fused_kernel(PackArgs a, int nbits)
     }
     if (e == 0) a.offsets[a.E] = tot5[0];
     if (a.lists.count != nullptr) {
-        if (e < a.E && total > 0) emit_items(a.lists, e, off, total, ex[1], ex[2], ex[3], ex[4]);
+        if (e < a.E && total > 0) emit_items(a.lists, e, off, total, ex[1], ex[2], ex[3], ex[4], total);
         if (e == 0) {
             a.lists.count[kListT128] = tot5[1];
             a.lists.count[kListT64] = tot5[2];

@@ -1794,10 +1794,20 @@ ek_status ek_layer_experts_forward(ek_layer *layer, int32_t n_calls, const int32
                     row0 += n;
                     continue;
                 }
+                if (layer->act8 && n > 16) {
+                    const int cut = ek::q8_items(n);
+                    for (int t = 0; t < cut; ++t) {
+                        int first, rows_t;
+                        ek::q8_item(n, cut, t, &first, &rows_t);
+                        items[ek::kListT128].push_back(ek::WorkItem{experts[i], (int32_t)row0 + first, rows_t, 0});
+                    }
+                    row0 += n;
+                    continue;
+                }
                 for (int32_t t = 0; t < full; ++t)
                     items[ek::kListT128].push_back(ek::WorkItem{experts[i], (int32_t)row0 + t * 128, 128, 0});
                 const ek::WorkItem rem{experts[i], (int32_t)row0 + full * 128, r, 0};
-                if (r > 64 || (layer->act8 && n > 16 && r > 0)) items[ek::kListT128].push_back(rem);
+                if (r > 64) items[ek::kListT128].push_back(rem);
                 else if (r > 32) items[ek::kListT64].push_back(rem);
                 else if (r > 16) items[ek::kListT32].push_back(rem);
                 else if (r > 0) items[ek::kListStream].push_back(rem);

@@ -16,9 +16,9 @@ namespace ek {
 
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ i32x4 signed8(uint4 u)
+__device__ __forceinline__ i32x4 signed8(uint4 u, uint32_t flip = 0x80808080u)
 {
-    return i32x4{(int)(u.x ^ 0x80808080u), (int)(u.y ^ 0x80808080u), (int)(u.z ^ 0x80808080u), (int)(u.w ^ 0x80808080u)};
+    return i32x4{(int)(u.x ^ flip), (int)(u.y ^ flip), (int)(u.z ^ flip), (int)(u.w ^ flip)};
 }
 
 // Four consecutive channels ch .. ch+3 of one output row.
@@ -174,19 +174,19 @@ __global__ __launch_bounds__(64 * kQ8Slices) void q8_stream_kernel(Q8Args a, int
 }
 
 
-// ---- tile kernel: items of up to 128 rows -------------------------------------------------------------
+// ---- tile kernel: items of up to 256 rows -------------------------------------------------------------
 //
-// One workgroup of four wavefronts: RB*32 rows x 4*64 matrix channels (stage 1: 128 hidden channels, up and
-// gate of each); every wave keeps all the rows and 64 channels.  MFMA 32x32x32 i8, weights as the A
-// operand.  Steps of 128 contraction elements:
+// One workgroup of four wavefronts, one per SIMD: RB*32 rows x 4*64 matrix channels (stage 1: 128 hidden
+// channels, up and gate of each); every wave keeps all the rows and 64 channels (256 rows: 256
+// accumulator registers).  MFMA 32x32x32 i8, weights as the A operand.  Steps of 128 contraction elements:
 //   - weights go from memory straight into registers, no other wave wants them: a 16-byte load per lane
-//     from the chunked layout is an A operand, loaded one step ahead into the registers its predecessor has
-//     just left;
-//   - the rows' bytes are shared by the four waves: LDS-DMA into three stages (two steps ahead), rows of 128
-//     bytes whose 16-byte pieces are XOR-swizzled so that fragment reads are conflict free.
-// Per step and workgroup the LDS takes 16 KiB and gives 64 KiB against 1024 cycles of MFMA (128 rows): half
-// its bandwidth.  Two workgroups fit a CU (registers: 256 per lane), so that one's epilogue and first loads
-// hide behind the other's products.
+//     from the chunked layout is an A operand.  A step's registers are loaded again as soon as they have been
+//     used, for the third step after it;
+//   - the rows' bytes are shared by the four waves: LDS-DMA into three stages (three steps ahead), rows of
+//     128 bytes whose 16-byte pieces are XOR-swizzled so that fragment reads are conflict free.
+// Per step of 256 rows and workgroup the vector L1 moves 64 KiB and the LDS 160 KiB against 2048 cycles of MFMA: half of
+// what the one and 60 % of what the other can.  (128 rows per wave, two workgroups per CU, wants 96 KiB of the L1: it was
+// the bound.  8192 x 8192 x 8192 on MI355X: 1.84 POP/s, and 2.73 with the weight loads taken out.)
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ void dma16(const void *gaddr, uint32_t lds_addr)     // lane l's 16 bytes land at lds_addr + 16 l
@@ -198,10 +198,12 @@ template <int N> __device__ __forceinline__ void wait_vmcnt() { asm volatile("s_
 __device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
 constexpr int kQ8Waves = 4, kQ8Stages = 3;
-constexpr int kQ8Stage = 128 * 128;                       // bytes of a stage: 128 rows x 128 elements
+constexpr int kQ8Stage = kQ8Rows * 128;                   // bytes of a stage: 256 rows x 128 elements
 constexpr int kQ8ScratchPitch = 64 * 2 + 16;              // epilogue: 32 rows x 64 channels of a wave
 constexpr int kQ8Scratch = 32 * kQ8ScratchPitch;
-constexpr int kQ8Lds = kQ8Stages * kQ8Stage + kQ8Waves * kQ8Scratch;
+constexpr int kQ8Scales = kQ8Stages * kQ8Stage + kQ8Waves * kQ8Scratch;   // then the scales: rows, channels, bias
+constexpr int kQ8Lds = kQ8Scales + 3 * 256 * 4;
+static_assert(kQ8Rows == 64 * kQ8Waves && 4 * 64 == 64 * kQ8Waves, "one row and one channel scale per thread");
 
 __device__ __forceinline__ int q8_key(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
@@ -214,6 +216,7 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
     const int l32 = lane & 31, kh = lane >> 5, j = lane & 15;
     const int KT = a.Kdim >> 6, nfull = KT >> 1, ns = (KT + 1) >> 1;
     const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
+    constexpr int kStep = 2 * NMAT * kChunkBytes;            // bytes from one step's weights to the next's
     // the wave's first 16-channel tile; block cb: matrix cb of tiles nt0, nt0 + 1, or tiles nt0 + 2 cb, + 1
     const int nt0 = (cblock * kQ8Waves + wave) * (NMAT == 2 ? 2 : 4);
     const uint8_t *wp[2];
@@ -234,11 +237,16 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
         xsrc[i] = a.x + row * a.Kdim + piece * 16;
         tail_fix[i] = (piece & 4) ? 64 : 0;
     }
-    float xs[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int rr = min(rb * 32 + l32, n - 1);
-        xs[rb] = a.x_scale[a.rows ? (int64_t)a.rows[row0 + rr] : (int64_t)(row0 + rr)];
+    // scales of the tile's rows and of its matrix channels, for the epilogue: one of each per thread, by way of LDS
+    float *scales = (float *)(lds + kQ8Scales);
+    float sc_row, sc_ch, sc_bias = 0.f;
+    {
+        const int rr = min(tid, n - 1);
+        sc_row = a.x_scale[a.rows ? (int64_t)a.rows[row0 + rr] : (int64_t)(row0 + rr)];
+        const int ch0 = cblock * kQ8Waves * (NMAT == 2 ? 32 : 64);          // up: threads 0 .. 127, gate: 128 .. 255
+        const int ch = min(ch0 + (NMAT == 2 ? tid & 127 : tid), a.NT * 16 - 1);
+        sc_ch = (NMAT == 2 ? (tid < 128 ? slab.s_up : slab.s_gate) : slab.s_down)[ch];
+        if (NMAT == 1 && a.bias) sc_bias = a.bias[ch];
     }
     const int bkey = q8_key(l32);
     int boff[4];
@@ -260,65 +268,97 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
         for (int i = 0; i < RB; ++i)
             dma16(xsrc[i] + (int64_t)sc * 128 - (sc == nfull ? tail_fix[i] : 0), lds_base + stage * kQ8Stage + (wave * RB + i) * 1024);
     };
-    uint4 w[4][2];
+    constexpr int D = kQ8Stages;
+    uint4 w[D][4][2];
     // one k-group's weights of the step wp points to; hi: from there to the step's second chunk
-    auto load_w = [&](int kg, int hi) {
+    auto load_w = [&](int slot, int kg, int hi) {
 #pragma unroll
-        for (int cb = 0; cb < 2; ++cb) w[kg][cb] = ldg16(wp[cb] + (kg >= 2 ? hi : 0) + (kg & 1) * 512);
+        for (int cb = 0; cb < 2; ++cb) w[slot][kg][cb] = ldg16(wp[cb] + (kg >= 2 ? hi : 0) + (kg & 1) * 512);
     };
-    // KGS k-groups of a step; REFILL: their weight registers are loaded again, for the step wp points to.  The
-    // fences keep the compiler from gathering the loads at the end of the step, and from converting all
-    // weights at its start (which would wait for the last of them).
-    auto body = [&](int stage, int hi, auto kgs_c, auto refill_c) {
-        constexpr int KGS = decltype(kgs_c)::value;
-        constexpr bool REFILL = decltype(refill_c)::value;
-        const uint8_t *st = lds + stage * kQ8Stage;
-        i32x4 b[2][RB];
+    // wp moves on to step s (which stays the last one where there is no step s); returns its `hi`
+    auto move_w = [&](int s) {
+        const int adv = s < ns ? kStep : 0;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) b[0][rb] = *(const i32x4 *)(st + boff[0] + rb * 4096);
+        for (int cb = 0; cb < 2; ++cb) wp[cb] += adv;
+        return s >= nfull && nfull < ns ? 0 : NMAT * kChunkBytes;   // half a step at the end: its one chunk twice
+    };
+    i32x4 b[2][RB];
+    auto read_b = [&](int stage, int kg) {
 #pragma unroll
-        for (int kg = 0; kg < KGS; ++kg) {
-            if (kg + 1 < KGS) {
+        for (int rb = 0; rb < RB; ++rb) b[kg & 1][rb] = *(const i32x4 *)(lds + stage * kQ8Stage + boff[kg] + rb * 4096);
+    };
+    auto products = [&](int slot, int kg) {
+        // a value of this place: the compiler would otherwise convert a loop-carried operand right behind its load
+        uint32_t flip = 0x80808080u;
+        asm volatile("" : "+s"(flip));
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb) b[(kg + 1) & 1][rb] = *(const i32x4 *)(st + boff[kg + 1] + rb * 4096);
+        for (int cb = 0; cb < 2; ++cb) {
+            const i32x4 q = signed8(w[slot][kg][cb], flip);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+                acc[rb][cb] = __builtin_amdgcn_mfma_i32_32x32x32_i8(q, b[kg & 1][rb], acc[rb][cb], 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int t = 0; t < D; ++t) {
+        issue(t, t);
+        const int hi = t == 0 ? NMAT * kChunkBytes : move_w(t);              // (K >= 128: the first step is whole)
+#pragma unroll
+        for (int kg = 0; kg < 4; ++kg) {
+            load_w(t, kg, hi);
+            __builtin_amdgcn_sched_barrier(0);       // in the order in which they are used
+        }
+    }
+    scales[tid] = sc_row;
+    scales[256 + tid] = sc_ch;
+    if (NMAT == 1) scales[512 + tid] = sc_bias;
+    wait_vmcnt<(D - 1) * RB + 8 * D>();   // step 0's DMAs have landed: everything else is younger
+    block_barrier();
+    read_b(0, 0);
+
+    // Step s (slot = stage = s % 3), one k-group after the other: the rows' fragments of the next k-group are read, the
+    // products of this one run, its weight registers are loaded for step s + 3.  Before the last k-group, whose
+    // fragments have been read, the workgroup meets: every wave is done with this stage, which takes step s + 3,
+    // and step s + 1 is in LDS, whose first fragments are read behind the last k-group's products.  A step's DMAs are
+    // followed by at least RB + 16 younger loads when they are waited for: every step issues the same number of loads,
+    // those for steps past the last repeat what is there.  The fences keep the compiler from gathering the loads at the
+    // end of the step, and from converting all weights at its start (which would wait for the last of them).
+    auto step = [&](int s, auto slot_c) {
+        constexpr int SLOT = decltype(slot_c)::value, NEXT = (SLOT + 1) % D;
+        const int hi = move_w(s + D);
+#pragma unroll
+        for (int kg = 0; kg < 4; ++kg) {
+            if (kg == 3) {
+                wait_vmcnt<(D - 2) * (RB + 8) + 8>();
+                block_barrier();
+                issue(s + D, SLOT);
+                read_b(NEXT, 0);
+            } else {
+                read_b(SLOT, kg + 1);
             }
-#pragma unroll
-            for (int cb = 0; cb < 2; ++cb) {
-                const i32x4 q = signed8(w[kg][cb]);
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
-                    acc[rb][cb] = __builtin_amdgcn_mfma_i32_32x32x32_i8(q, b[kg & 1][rb], acc[rb][cb], 0, 0, 0);
-            }
-            if (REFILL) load_w(kg, hi);
+            if (kg < 2 || s < nfull) products(SLOT, kg);             // half a step at the end has two k-groups
+            load_w(SLOT, kg, hi);
+            __builtin_amdgcn_sched_group_barrier(0x100, RB, 0);      // the LDS reads first
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * RB, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    issue(0, 0);
-    issue(1, 1);
-#pragma unroll
-    for (int kg = 0; kg < 4; ++kg) load_w(kg, NMAT * kChunkBytes);           // (K >= 128: the first step is whole)
-
-    // At the start of step s this wave's DMAs of the step have landed when no more than the loads younger than them are
-    // outstanding: the DMAs of step s + 1 and one step's weights.  Every step issues the same number of loads; those for
-    // steps past the last one repeat what is there (half a step at the end: its one chunk twice).
-    int stage = 0, s = 0;
-    auto open = [&] {
-        wait_vmcnt<RB + 8>();
-        block_barrier();              // everyone's rows are there, and the stage of step s - 1 is free
-        issue(s + 2, stage == 0 ? 2 : stage - 1);
+    // D steps a round (the loop has no other way out, so that the compiler's own waits are those of a full ring)
+    auto steps = [&](auto self, int s, auto slot_c) -> void {
+        constexpr int SLOT = decltype(slot_c)::value;
+        step(s, slot_c);
+        if constexpr (SLOT + 1 < D) self(self, s + 1, std::integral_constant<int, SLOT + 1>{});
     };
-    for (; s < nfull; ++s) {
-        open();
-        const int adv = s + 1 < ns ? 2 * NMAT * kChunkBytes : 0;
-#pragma unroll
-        for (int cb = 0; cb < 2; ++cb) wp[cb] += adv;
-        body(stage, s + 1 == nfull && nfull < ns ? 0 : NMAT * kChunkBytes, std::integral_constant<int, 4>{}, std::true_type{});
-        stage = stage == 2 ? 0 : stage + 1;
-    }
-    if (nfull < ns) {
-        open();
-        body(stage, 0, std::integral_constant<int, 2>{}, std::false_type{});
-    }
+    auto rest = [&](auto self, int s, auto slot_c) -> void {
+        constexpr int SLOT = decltype(slot_c)::value;
+        if (s >= ns) return;
+        step(s, slot_c);
+        if constexpr (SLOT + 2 < D) self(self, s + 1, std::integral_constant<int, SLOT + 1>{});
+    };
+    int s = 0;
+    for (; s + D <= ns; s += D) steps(steps, s, std::integral_constant<int, 0>{});
+    rest(rest, s, std::integral_constant<int, 0>{});
     wait_vmcnt<0>();                  // the repeated loads
 
     // Epilogue.  Register 4 q + r of a lane: channel 8 q + 4 kh + r of its block, row l32 of row block rb.  The values
@@ -330,36 +370,46 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
     constexpr int PPR = NC / 8;                                  // 16-byte pieces per row
     const bool whole = nch == NC && (a.out_stride & 7) == 0;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    float ws[2][16];
+    float ws[2][16], bias[2][16];
 #pragma unroll
     for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int nt = min(nt0 + (NMAT == 2 ? 0 : cb * 2) + (q >> 1), a.NT - 1);
-            const float *sp = (NMAT == 2 ? (cb == 0 ? slab.s_up : slab.s_gate) : slab.s_down) + nt * 16 + (q & 1) * 8 + kh * 4;
+            const float *sp = scales + 256 + (NMAT == 2 ? cb * 128 + wave * 32 : wave * 64 + cb * 32) + q * 8 + kh * 4;
             const float4 v = *(const float4 *)sp;
             ws[cb][q * 4] = v.x; ws[cb][q * 4 + 1] = v.y; ws[cb][q * 4 + 2] = v.z; ws[cb][q * 4 + 3] = v.w;
+            if (NMAT == 1) {
+                const float4 t = *(const float4 *)(sp + 256);
+                bias[cb][q * 4] = t.x; bias[cb][q * 4 + 1] = t.y; bias[cb][q * 4 + 2] = t.z; bias[cb][q * 4 + 3] = t.w;
+            }
         }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        if (rb * 32 >= n) break;
+        const float xs = scales[rb * 32 + l32];
 #pragma unroll
         for (int cb = 0; cb < (NMAT == 2 ? 1 : 2); ++cb)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                T4 o;
+                float v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = q * 4 + r;
-                    if constexpr (NMAT == 2) {
-                        o[r] = swiglu_rounded<T>(as_fp32((float)acc[rb][0][i] * (xs[rb] * ws[0][i])),
-                                                 as_fp32((float)acc[rb][1][i] * (xs[rb] * ws[1][i])));
-                    } else {
-                        float v = as_fp32((float)acc[rb][cb][i] * (xs[rb] * ws[cb][i]));
-                        const int ch = c0 + cb * 32 + q * 8 + kh * 4 + r;
-                        if (a.bias && ch < a.N) v += a.bias[ch];
-                        o[r] = (T)v;
+                    v[r] = as_fp32((float)acc[rb][cb][i] * (xs * ws[cb][i]));
+                }
+                T4 o;
+                if constexpr (NMAT == 2) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int i = q * 4 + r;
+                        o[r] = swiglu_rounded<T>(v[r], as_fp32((float)acc[rb][1][i] * (xs * ws[1][i])));
                     }
+                } else {
+                    if (a.bias) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] += bias[cb][q * 4 + r];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = (T)v[r];
                 }
                 *(T4 *)(scratch + l32 * kQ8ScratchPitch + (cb * 32 + q * 8 + kh * 4) * 2) = o;
             }
@@ -385,36 +435,43 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
     }
 }
 
-// Tiles are numbered item by item; XCD x (workgroups x, x + 8, ...) walks a contiguous eighth of them, so that
-// the workgroups that share an item's rows or an expert's weights share an L2.
+// Tiles are numbered in groups of `group` items, channel block by channel block within a group; XCD x (workgroups
+// x, x + 8, ...) walks a contiguous eighth of them, so that the workgroups that share an item's rows or an expert's
+// weights run side by side on one L2.
 template <typename T, int NMAT>
-__global__ __launch_bounds__(64 * kQ8Waves, 2) void q8_tile_kernel(Q8Args a, int cblocks)
+__global__ __launch_bounds__(64 * kQ8Waves, 1) void q8_tile_kernel(Q8Args a, int cblocks, int group)
 {
     extern __shared__ __align__(1024) uint8_t q8_lds[];
-    const int items = a.dense_rows > 0 ? (int)((a.dense_rows + 127) >> 7) : a.lists.count[kListT128];
-    const int64_t tiles = (int64_t)items * cblocks;
-    const int64_t per = (tiles + 7) >> 3, at = blockIdx.x >> 3;
-    const int64_t tile = (int64_t)(blockIdx.x & 7) * per + at;
+    // (what names the tile is the same for every lane: scalar loads)
+    typedef const __attribute__((address_space(4))) int32_t *cint;
+    typedef const __attribute__((address_space(4))) uint64_t *cptr;
+    const uint32_t items = a.dense_rows > 0 ? (uint32_t)((a.dense_rows + kQ8Rows - 1) / kQ8Rows) : (uint32_t)((cint)(uintptr_t)a.lists.count)[kListT128];
+    const uint32_t tiles = items * (uint32_t)cblocks, per = (tiles + 7) >> 3, at = blockIdx.x >> 3;
+    const uint32_t tile = (blockIdx.x & 7) * per + at;
     if (at >= per || tile >= tiles) return;
-    const int it = (int)(tile / cblocks), cblock = (int)(tile - (int64_t)it * cblocks);
+    const uint32_t in_full = (uint32_t)group * cblocks, g = tile / in_full, rem = tile - g * in_full;
+    const uint32_t in_group = min((uint32_t)group, items - g * group);
+    const int cblock = (int)(rem / in_group), it = (int)(g * group + rem % in_group);
     int e = 0, row0, n;
     if (a.dense_rows > 0) {
-        row0 = it * 128;
-        n = (int)min((int64_t)128, a.dense_rows - row0);
+        row0 = it * kQ8Rows;
+        n = (int)min((int64_t)kQ8Rows, a.dense_rows - row0);
     } else {
-        const WorkItem item = a.lists.items[kListT128][it];
-        e = item.expert; row0 = item.row0; n = item.nrows;
+        const cint item = (cint)(uintptr_t)(a.lists.items[kListT128] + it);
+        e = item[0]; row0 = item[1]; n = item[2];
     }
-    e = __builtin_amdgcn_readfirstlane(e);
-    row0 = __builtin_amdgcn_readfirstlane(row0);
-    n = __builtin_amdgcn_readfirstlane(n);
-    const ExpertSlab slab = a.slabs[e];
+    const cptr sp = (cptr)(uintptr_t)(a.slabs + e);
+    const ExpertSlab slab{(const uint8_t *)sp[0], (const uint8_t *)sp[1], (const float *)sp[2], (const float *)sp[3], (const float *)sp[4]};
     if ((NMAT == 2 ? slab.upgate : slab.down) == nullptr) return;          // expert not loaded: the call has been flagged
     switch ((n + 31) >> 5) {
     case 1: q8_tile<T, NMAT, 1>(a, slab, row0, n, cblock, q8_lds); break;
     case 2: q8_tile<T, NMAT, 2>(a, slab, row0, n, cblock, q8_lds); break;
     case 3: q8_tile<T, NMAT, 3>(a, slab, row0, n, cblock, q8_lds); break;
-    default: q8_tile<T, NMAT, 4>(a, slab, row0, n, cblock, q8_lds); break;
+    case 4: q8_tile<T, NMAT, 4>(a, slab, row0, n, cblock, q8_lds); break;
+    case 5: q8_tile<T, NMAT, 5>(a, slab, row0, n, cblock, q8_lds); break;
+    case 6: q8_tile<T, NMAT, 6>(a, slab, row0, n, cblock, q8_lds); break;
+    case 7: q8_tile<T, NMAT, 7>(a, slab, row0, n, cblock, q8_lds); break;
+    default: q8_tile<T, NMAT, 8>(a, slab, row0, n, cblock, q8_lds); break;
     }
 }
 
@@ -424,8 +481,9 @@ static hipError_t launch_tiles(const Q8Args &a, int64_t max_items, hipStream_t s
     const int per = NMAT == 2 ? 2 * kQ8Waves : 4 * kQ8Waves;    // 16-channel tiles per workgroup
     const int cblocks = (a.NT + per - 1) / per;
     const int64_t tiles = max_items * cblocks, grid = (tiles + 7) / 8 * 8;
-    if (grid > (int64_t)1 << 23) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((q8_tile_kernel<T, NMAT>), dim3((unsigned)grid), dim3(64 * kQ8Waves), kQ8Lds, s, a, cblocks);
+    if (grid >= (int64_t)1 << 24) return hipErrorInvalidValue;          // threads of a launch
+    hipLaunchKernelGGL((q8_tile_kernel<T, NMAT>), dim3((unsigned)grid), dim3(64 * kQ8Waves), kQ8Lds, s, a, cblocks,
+                       a.dense_rows > 0 ? 4 : 1);
     return hipGetLastError();
 }
 
@@ -458,7 +516,7 @@ template <typename T> static hipError_t launch_dense_t(const Q8Args &a, hipStrea
     const dim3 block(64 * kQ8Slices);
     if (n <= 16) hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 1, 2>), dim3((unsigned)a.NT, 1), block, 0, s, a, 0, 16);
     else if (n <= 128) hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 4, 2>), dim3((unsigned)a.NT, (unsigned)((n + 63) / 64)), block, 0, s, a, 0, 64);
-    else return launch_tiles<T, 1>(a, (n + 127) / 128, s);
+    else return launch_tiles<T, 1>(a, (n + kQ8Rows - 1) / kQ8Rows, s);
     return hipGetLastError();
 }
 

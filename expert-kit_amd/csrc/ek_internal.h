@@ -59,11 +59,12 @@ enum { kListStream = 0, kListT32 = 1, kListT64 = 2, kListT128 = 3, kNumLists = 4
 struct WorkLists {
     WorkItem *items[kNumLists];
     int32_t *count;              // [kNumLists]
-    // 1: a segment of more than 16 rows goes into the 128-row list whole, its remainder of any length included
-    // (layers on 8-bit activations, whose tile kernel takes items of 1 .. 128 rows)
+    // 1: a segment of more than 16 rows goes into the 128-row list whole, in as few items of at most kQ8Rows rows as
+    // hold it, cut evenly in blocks of 32 rows (layers on 8-bit activations, whose tile kernel takes 1 .. kQ8Rows rows)
     int32_t one_class = 0;
 };
 constexpr int kWideRows = 64;
+constexpr int kQ8Rows = 256;
 // tile_items: work items the ordinary cut would give the tile kernel; one of them spreads
 // over ceil(inter / 128) workgroups in stage 1 (the tile kernel's narrow form, which such calls
 // get), and below half a chip of them the call takes as long as one tile's two contractions
@@ -83,11 +84,22 @@ inline bool wide_cut_pays(int64_t tile_items, int64_t rows, int64_t hidden, int6
 }
 inline int64_t list_capacity(int list, int64_t P, int64_t E, bool one_class = false)
 {
-    if (one_class && list != kListStream) return list == kListT128 ? P / 128 + (P / 17 < E ? P / 17 : E) : 0;
+    if (one_class && list != kListStream) return list == kListT128 ? P / kQ8Rows + (P / 17 < E ? P / 17 : E) : 0;
     const int64_t min_rows[kNumLists] = {1, 17, 33, 65};
     const int64_t by_rows = P / min_rows[list];
     if (list == kListT128) return by_rows;
     return by_rows < E ? by_rows : E;
+}
+
+// Item i of the one-class cut of a segment of n rows (n > 16) into `items`: its first row and its rows.
+constexpr int q8_items(int n) { return (n + kQ8Rows - 1) / kQ8Rows; }
+__host__ __device__ inline void q8_item(int n, int items, int i, int *first, int *rows)
+{
+    const int blocks = (n + 31) >> 5, base = blocks / items, more = blocks % items;
+    const int b0 = i * base + (i < more ? i : more);
+    *first = b0 * 32;
+    const int end = (b0 + base + (i < more)) * 32;
+    *rows = (end < n ? end : n) - *first;
 }
 
 // ---- router (logits -> ids, gate weights) -------------------------------------

@@ -104,7 +104,7 @@ __device__ __forceinline__ SegmentCut cut_segment(int32_t n, int32_t one_class)
 {
     SegmentCut c;
     if (one_class) {
-        c.n128 = n > 16 ? (n + 127) >> 7 : 0;
+        c.n128 = n > 16 ? q8_items(n) : 0;
         c.n64 = c.n32 = 0;
         c.ns = n > 0 && n <= 16;
         return c;
@@ -116,14 +116,24 @@ __device__ __forceinline__ SegmentCut cut_segment(int32_t n, int32_t one_class)
     c.ns = r > 0 && r <= 16;
     return c;
 }
-// items of rows seg0 .. seg0+n-1, which end a segment of seg_n rows
-__device__ __forceinline__ void emit_items(const WorkLists &l, int32_t e, int32_t seg0, int32_t n,
-                                           int32_t p128, int32_t p64, int32_t p32, int32_t ps, int32_t seg_n)
+__device__ __forceinline__ WorkItem q8_work_item(int32_t e, int32_t seg0, int32_t n, int32_t items, int32_t i)
 {
+    int32_t first, rows;
+    q8_item(n, items, i, &first, &rows);
+    return WorkItem{e, seg0 + first, rows, 0};
+}
+__device__ __forceinline__ void emit_items(const WorkLists &l, int32_t e, int32_t seg0, int32_t n,
+                                           int32_t p128, int32_t p64, int32_t p32, int32_t ps)
+{
+    if (l.one_class && n > 16) {
+        const int32_t items = q8_items(n);
+        for (int32_t i = 0; i < items; ++i) l.items[kListT128][p128 + i] = q8_work_item(e, seg0, n, items, i);
+        return;
+    }
     const int32_t full = n >> 7, r = n & 127;
     for (int32_t t = 0; t < full; ++t) l.items[kListT128][p128 + t] = WorkItem{e, seg0 + t * 128, 128, 0};
     const WorkItem rem{e, seg0 + full * 128, r, 0};
-    if (r > 64 || (l.one_class && seg_n > 16 && r > 0)) l.items[kListT128][p128 + full] = rem;
+    if (r > 64) l.items[kListT128][p128 + full] = rem;
     else if (r > 32) l.items[kListT64][p64] = rem;
     else if (r > 16) l.items[kListT32][p32] = rem;
     else if (r > 0) l.items[kListStream][ps] = rem;
@@ -169,7 +179,7 @@ __global__ __launch_bounds__(1024) void pack_scan_kernel(PackArgs a)
     const int32_t p64 = block_exclusive_scan(c.n64, wave_tot, &s64);
     const int32_t p32 = block_exclusive_scan(c.n32, wave_tot, &s32);
     const int32_t ps = block_exclusive_scan(c.ns, wave_tot, &ss);
-    if (e < a.E && total > 0) emit_items(a.lists, e, off, total, p128, p64, p32, ps, total);
+    if (e < a.E && total > 0) emit_items(a.lists, e, off, total, p128, p64, p32, ps);
     if (e == 0) {
         a.lists.count[kListT128] = s128;
         a.lists.count[kListT64] = s64;
@@ -199,9 +209,13 @@ __global__ __launch_bounds__(256) void segment_lists_kernel(WorkLists l, int32_t
     }
     const SegmentCut c = cut_segment(n, l.one_class);
     const int32_t full = n >> 7;
-    for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][t] = WorkItem{e, row0 + t * 128, 128, 0};
+    if (l.one_class && n > 16) {
+        for (int32_t t = threadIdx.x; t < c.n128; t += 256) l.items[kListT128][t] = q8_work_item(e, row0, n, c.n128, t);
+    } else {
+        for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][t] = WorkItem{e, row0 + t * 128, 128, 0};
+        if (threadIdx.x == 0 && (n & 127)) emit_items(l, e, row0 + full * 128, n & 127, full, 0, 0, 0);    // the remainder, into its class
+    }
     if (threadIdx.x == 0) {
-        if (n & 127) emit_items(l, e, row0 + full * 128, n & 127, full, 0, 0, 0, n);    // the remainder, into its class
         l.count[kListT128] = c.n128;
         l.count[kListT64] = c.n64;
         l.count[kListT32] = c.n32;
@@ -230,10 +244,14 @@ __global__ __launch_bounds__(256) void append_segment_kernel(WorkLists l, int32_
     }
     const SegmentCut c = cut_segment(n, l.one_class);
     const int32_t full = n >> 7, r = n & 127;
-    for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][p128 + t] = WorkItem{e, row0 + t * 128, 128, 0};
     for (int32_t t = threadIdx.x; t < n; t += 256) row_token[row0 + t] = t;
+    if (l.one_class && n > 16) {
+        for (int32_t t = threadIdx.x; t < c.n128; t += 256) l.items[kListT128][p128 + t] = q8_work_item(e, row0, n, c.n128, t);
+    } else {
+        for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][p128 + t] = WorkItem{e, row0 + t * 128, 128, 0};
+        if (threadIdx.x == 0 && r > 0) emit_items(l, e, row0 + full * 128, r, p128 + full, p64, p32, ps);
+    }
     if (threadIdx.x == 0) {
-        if (r > 0) emit_items(l, e, row0 + full * 128, r, p128 + full, p64, p32, ps, n);
         l.count[kListT128] = p128 + c.n128;
         l.count[kListT64] = p64 + c.n64;
         l.count[kListT32] = p32 + c.n32;
@@ -369,7 +387,7 @@ __global__ __launch_bounds__(1024) void pack_fused_kernel(PackArgs a, int nbits)
     }
     if (e == 0) a.offsets[a.E] = tot5[0];
     if (a.lists.count != nullptr) {
-        if (e < a.E && total > 0) emit_items(a.lists, e, off, total, ex[1], ex[2], ex[3], ex[4], total);
+        if (e < a.E && total > 0) emit_items(a.lists, e, off, total, ex[1], ex[2], ex[3], ex[4]);
         if (e == 0) {
             a.lists.count[kListT128] = tot5[1];
             a.lists.count[kListT64] = tot5[2];

@@ -897,6 +897,15 @@ ek_status copy_route_out(ek_layer *L, const Workspace &W, const ek_route_out *r,
     return EK_OK;
 }
 
+// The work lists of a layer call of P pairs (the same cut for pack, an appended shared segment and the launches).
+int one_class_of(const ek_layer *L, int64_t P) { return L->act8 ? ek::q8_one_class(P, L->cfg.n_experts) : 0; }
+ek::WorkLists lists_of(const ek_layer *L, const Workspace &W, int64_t P)
+{
+    ek::WorkLists l = W.lists;
+    l.one_class = one_class_of(L, P);
+    return l;
+}
+
 ek::PackArgs pack_args(ek_layer *L, const Workspace &W, const int32_t *ids, int64_t P, bool check_loaded)
 {
     ek::PackArgs a;
@@ -915,7 +924,7 @@ ek::PackArgs pack_args(ek_layer *L, const Workspace &W, const int32_t *ids, int6
     a.err = W.err;
     a.activation = check_loaded ? L->d_activation : nullptr;
     a.tile_items_host = check_loaded ? L->d_tile_items : nullptr;
-    if (check_loaded) a.lists = W.lists;
+    if (check_loaded) a.lists = lists_of(L, W, P);
     else a.lists = ek::WorkLists{{nullptr, nullptr, nullptr, nullptr}, nullptr};
     return a;
 }
@@ -1008,11 +1017,11 @@ ek_status enqueue_ffn_q8(ek_layer *L, const Workspace &W, const uint8_t *x, cons
 // segment); they get launches of their own on the side stream, beside the others.
 // exact: the lists' lengths when the caller built them on the host (the grids then fit them,
 // an empty list gets no launch, and the two chains run side by side exactly when both have work).
-// x_scale (EK_CFG_ACT8): x are int8 rows with these scales, the lists cover h_rows packed rows.
+// x_scale (EK_CFG_ACT8): x are int8 rows with these scales, the lists cover h_rows packed rows, cut with one_class.
 ek_status enqueue_ffn(ek_layer *L, const Workspace &W, const void *x, const int32_t *rows, void *out, int64_t P, int64_t E,
                       hipStream_t s, hipEvent_t *ev, int64_t wide_items = 0, int64_t extra_stream = 0,
                       int64_t shared_wide = 0, const int64_t *exact = nullptr, int64_t known_tile_items = -1,
-                      const float *x_scale = nullptr, int64_t h_rows = 0)
+                      const float *x_scale = nullptr, int64_t h_rows = 0, int one_class = 0)
 {
     const int64_t H = L->cfg.hidden, I = L->cfg.inter;
     ek::FfnArgs a1;
@@ -1023,7 +1032,7 @@ ek_status enqueue_ffn(ek_layer *L, const Workspace &W, const void *x, const int3
     a2.N = (int32_t)H; a2.Kdim = (int32_t)I;
     int64_t cap[ek::kNumLists];
     for (int l = 0; l < ek::kNumLists; ++l) {
-        cap[l] = ek::list_capacity(l, P, E, L->act8) + (l == ek::kListStream ? extra_stream : 0);
+        cap[l] = ek::list_capacity(l, P, E, one_class) + (l == ek::kListStream ? extra_stream : 0);
         if (exact) cap[l] = exact[l];          // the caller built the lists on the host
         if (cap[l] > W.list_cap[l]) cap[l] = W.list_cap[l];
         if (cap[l] < 0) cap[l] = 0;
@@ -1155,7 +1164,7 @@ ek_status enqueue_route(ek_layer *L, const Workspace &W, const int32_t *ids, int
         own.count = W.wide_count;
         ek::launch_append_segment(own, E, (int32_t)P, (int32_t)T, W.row_token, 2, s);
     } else if (sc.shared) {
-        ek::launch_append_segment(W.lists, E, (int32_t)P, (int32_t)T, W.row_token, sc.streamed ? 1 : 0, s);
+        ek::launch_append_segment(lists_of(L, W, P), E, (int32_t)P, (int32_t)T, W.row_token, sc.streamed ? 1 : 0, s);
     }
     EK_HIP(hipGetLastError());
     return EK_OK;
@@ -1297,7 +1306,7 @@ ek_status enqueue_forward(ek_layer *L, const Workspace &W, const void *x, const 
         EK_TRY(enqueue_ffn(L, W, x, W.row_token, W.yp, in_lists ? P + T : P, in_lists ? E + 1 : E, s, ev, 0,
                            shared_streamed ? (T + 15) / 16 : 0,
                            shared_wide ? (T + ek::kWideRows - 1) / ek::kWideRows : 0, nullptr, -1,
-                           x_scale, in_lists || shared_wide ? P + T : P));
+                           x_scale, in_lists || shared_wide ? P + T : P, one_class_of(L, P)));
         if (sc.own) EK_HIP(hipStreamWaitEvent(s, L->ev_sjoin, 0));
         if (ev) EK_HIP(hipEventRecord(ev[3], s));
         if (before_combine) EK_TRY((*before_combine)());
@@ -1699,7 +1708,7 @@ ek_status ek_layer_expert_forward(ek_layer *layer, int32_t expert, const void *x
                 d_x = layer->ws.xq;
             }
             EK_TRY(enqueue_ffn(layer, layer->ws, d_x, nullptr, d_out, n, 1, s, nullptr, wide ? wide_items : 0, 0, 0, nullptr,
-                               wide ? 0 : (n >> 7) + ((n & 127) > 16), layer->ws.xq_scale, n));
+                               wide ? 0 : (n >> 7) + ((n & 127) > 16), layer->ws.xq_scale, n, layer->act8));
             if (layer->padded) EK_TRY(rows_out(layer, out, layer->st_y, n, mem, s));
             else if (mem == EK_HOST) EK_TRY(d2h(layer, out, layer->st_y, (size_t)n * H * 2, s));
         }
@@ -1922,7 +1931,7 @@ ek_status ek_layer_experts_forward(ek_layer *layer, int32_t n_calls, const int32
                 ffn_x = layer->ws.xq;
             }
             EK_TRY(enqueue_ffn(layer, layer->ws, ffn_x, nullptr, layer->st_y, P, n_calls, s, nullptr, wide ? wide_items : 0, 0, 0,
-                               wide ? nullptr : exact, -1, layer->ws.xq_scale, P));
+                               wide ? nullptr : exact, -1, layer->ws.xq_scale, P, layer->act8));
             EK_HIP(hipGetLastError());
             row0 = 0;
             if (one_transfer) {

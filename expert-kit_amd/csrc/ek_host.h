@@ -60,6 +60,7 @@ struct DeviceGuard {
     explicit DeviceGuard(int dev)
     {
         if (hipGetDevice(&prev) != hipSuccess) { (void)hipGetLastError(); prev = -1; }
+        if (prev == dev) { ok = true; prev = -1; return; }
         ok = hipSetDevice(dev) == hipSuccess;
         if (!ok) (void)hipGetLastError();
     }

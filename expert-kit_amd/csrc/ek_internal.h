@@ -60,7 +60,8 @@ struct WorkLists {
     WorkItem *items[kNumLists];
     int32_t *count;              // [kNumLists]
     // 1: a segment of more than 16 rows goes into the 128-row list whole, in as few items of at most kQ8Rows rows as
-    // hold it, cut evenly in blocks of 32 rows (layers on 8-bit activations, whose tile kernel takes 1 .. kQ8Rows rows)
+    // hold it, cut evenly in blocks of 32 rows (layers on 8-bit activations, whose tile kernel takes 1 .. kQ8Rows rows);
+    // 2: every segment does, however short
     int32_t one_class = 0;
 };
 constexpr int kWideRows = 64;
@@ -82,15 +83,23 @@ inline bool wide_cut_pays(int64_t tile_items, int64_t rows, int64_t hidden, int6
     const double streamed_us = (double)rows * (0.053 + 1.48e-8 * (double)hidden * (double)inter);
     return streamed_us < 0.92 * tile_call_us(hidden, inter);
 }
-inline int64_t list_capacity(int list, int64_t P, int64_t E, bool one_class = false)
+inline int64_t list_capacity(int list, int64_t P, int64_t E, int one_class = 0)
 {
-    if (one_class && list != kListStream) return list == kListT128 ? P / kQ8Rows + (P / 17 < E ? P / 17 : E) : 0;
+    if (one_class && list == kListT128) {
+        const int64_t segments = one_class == 2 ? P : P / 17;
+        return P / kQ8Rows + (segments < E ? segments : E);
+    }
+    if (one_class && (list != kListStream || one_class == 2)) return 0;
     const int64_t min_rows[kNumLists] = {1, 17, 33, 65};
     const int64_t by_rows = P / min_rows[list];
     if (list == kListT128) return by_rows;
     return by_rows < E ? by_rows : E;
 }
 
+// A layer on 8-bit activations whose call has more than 32 pairs per expert sends every segment to the tile kernel: most
+// are longer than the streaming kernel's 16 rows, and the streaming launch, a grid of (experts x channel tiles) that
+// finds next to nothing, costs more than the few short tiles (DeepSeek-V3 shape, 8192 tokens: 83 us of 4.3 ms).
+inline int q8_one_class(int64_t P, int64_t E) { return P > 32 * E ? 2 : 1; }
 // Item i of the one-class cut of a segment of n rows (n > 16) into `items`: its first row and its rows.
 constexpr int q8_items(int n) { return (n + kQ8Rows - 1) / kQ8Rows; }
 __host__ __device__ inline void q8_item(int n, int items, int i, int *first, int *rows)
@@ -230,6 +239,7 @@ struct RowQuantArgs {
     int32_t q_stride;         // a multiple of 8, at least H
     float eps;
     double inv_h;             // 1 / H
+    bool wide;                // norm: sum the squares in fp64 throughout (an eps below what fp32 squares resolve)
     bool vec;                 // rows of x start on 16-byte boundaries (H a multiple of 8)
 };
 hipError_t launch_row_quant(const RowQuantArgs &a, int act, bool norm, hipStream_t s);

@@ -104,9 +104,10 @@ __device__ __forceinline__ SegmentCut cut_segment(int32_t n, int32_t one_class)
 {
     SegmentCut c;
     if (one_class) {
-        c.n128 = n > 16 ? q8_items(n) : 0;
+        const bool tile = one_class == 2 ? n > 0 : n > 16;
+        c.n128 = tile ? q8_items(n) : 0;
         c.n64 = c.n32 = 0;
-        c.ns = n > 0 && n <= 16;
+        c.ns = n > 0 && !tile;
         return c;
     }
     const int32_t r = n & 127;
@@ -116,6 +117,7 @@ __device__ __forceinline__ SegmentCut cut_segment(int32_t n, int32_t one_class)
     c.ns = r > 0 && r <= 16;
     return c;
 }
+__device__ __forceinline__ bool in_one_class(const WorkLists &l, int32_t n) { return l.one_class == 2 ? n > 0 : l.one_class && n > 16; }
 __device__ __forceinline__ WorkItem q8_work_item(int32_t e, int32_t seg0, int32_t n, int32_t items, int32_t i)
 {
     int32_t first, rows;
@@ -125,7 +127,7 @@ __device__ __forceinline__ WorkItem q8_work_item(int32_t e, int32_t seg0, int32_
 __device__ __forceinline__ void emit_items(const WorkLists &l, int32_t e, int32_t seg0, int32_t n,
                                            int32_t p128, int32_t p64, int32_t p32, int32_t ps)
 {
-    if (l.one_class && n > 16) {
+    if (in_one_class(l, n)) {
         const int32_t items = q8_items(n);
         for (int32_t i = 0; i < items; ++i) l.items[kListT128][p128 + i] = q8_work_item(e, seg0, n, items, i);
         return;
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(256) void segment_lists_kernel(WorkLists l, int32_t
     }
     const SegmentCut c = cut_segment(n, l.one_class);
     const int32_t full = n >> 7;
-    if (l.one_class && n > 16) {
+    if (in_one_class(l, n)) {
         for (int32_t t = threadIdx.x; t < c.n128; t += 256) l.items[kListT128][t] = q8_work_item(e, row0, n, c.n128, t);
     } else {
         for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][t] = WorkItem{e, row0 + t * 128, 128, 0};
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(256) void append_segment_kernel(WorkLists l, int32_
     const SegmentCut c = cut_segment(n, l.one_class);
     const int32_t full = n >> 7, r = n & 127;
     for (int32_t t = threadIdx.x; t < n; t += 256) row_token[row0 + t] = t;
-    if (l.one_class && n > 16) {
+    if (in_one_class(l, n)) {
         for (int32_t t = threadIdx.x; t < c.n128; t += 256) l.items[kListT128][p128 + t] = q8_work_item(e, row0, n, c.n128, t);
     } else {
         for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][p128 + t] = WorkItem{e, row0 + t * 128, 128, 0};

@@ -14,211 +14,271 @@
 #include "ek_internal.h"
 #include "ek_mfma.h"
 
+#include <algorithm>
+
 namespace ek {
 
-// rint(127 p / m) for |p| <= m.  `up` is a power of two that brings a tiny m into the range of
-// normal numbers and inv = 127 / (m * up).  The fp32 product is within 2^-22 relative of the real
+// rint(127 p / m) for |p| <= m, as inv = 127 / m times p.  The fp32 product t is within 2^-22 relative of the real
 // value, so it decides unless it lies within 2^-15 of a half-integer; there 254 |p| is compared with the
 // odd multiple of m that the half-integer stands for, both exact in fp64 (24 + 8 bits).
-__device__ __forceinline__ bool quant_fast(float p, float inv, float up, float &k)
-{
-    const float t = (p * up) * inv;
-    k = __builtin_rintf(t);
-    return __builtin_fabsf(__builtin_fabsf(t - k) - 0.5f) > 0x1p-15f;   // decided
-}
-__device__ __forceinline__ float quant_exact(float p, float m, float inv, float up)
+//
+// Adding 1.5 * 2^23 rounds t to the nearest integer, ties to even, and leaves it in the low byte of the sum as the
+// two's complement code.
+constexpr float kToInt = 12582912.f;
+__device__ __forceinline__ uint32_t quant_exact(float p, float m, float inv)
 {
     const float a = __builtin_fabsf(p);
-    const float f = __builtin_floorf((a * up) * inv);
+    const float f = __builtin_floorf(a * inv);
     const double lhs = 254.0 * (double)a, rhs = (2.0 * (double)f + 1.0) * (double)m;
     const bool odd = ((int)f & 1) != 0;
-    const float k = lhs > rhs || (lhs == rhs && odd) ? f + 1.f : f;
-    return p < 0.f ? -k : k;
+    const int k = (int)f + (lhs > rhs || (lhs == rhs && odd) ? 1 : 0);
+    return (uint32_t)(p < 0.f ? -k : k);
 }
-
-// 8 consecutive values of a row from index i on (i < n); vec: 16-byte loads are possible
-template <typename T> __device__ __forceinline__ void load8(const T *row, int i, int n, bool vec, float *v)
+// 8 codes as bytes
+__device__ __forceinline__ uint2 quant8(const float *p, float m, float inv)
 {
-    typedef T V8 __attribute__((ext_vector_type(8)));
-    if (vec) {
-        const V8 x = *(const V8 *)(row + i);
+    uint32_t u[8];
+    float worst = 0.f;               // distance to the nearest integer: 1/2 on a border
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (float)x[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = i + j < n ? (float)row[i + j] : 0.f;
+    for (int j = 0; j < 8; ++j) {
+        const float t = p[j] * inv, s = t + kToInt;
+        worst = __builtin_fmaxf(worst, __builtin_fabsf(t - (s - kToInt)));
+        u[j] = __builtin_bit_cast(uint32_t, s);
     }
-}
-
-template <typename T> __device__ __forceinline__ void store8(T *row, int i, const float *v)
-{
-    typedef T V8 __attribute__((ext_vector_type(8)));
-    V8 o;
+    if (worst > 0.5f - 0x1p-15f) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = (T)v[j];
-    *(V8 *)(row + i) = o;
-}
-
-// The values to quantise of 8 columns of a row: p = sum * gain (NORM; `r` receives the rounded sum), or the
-// row itself.
-template <typename T, bool NORM>
-__device__ __forceinline__ void row_values(const RowQuantArgs &a, int64_t row, int i, float *p, float *r)
-{
-    load8<T>((const T *)a.x + row * a.H, i, a.H, a.vec, p);
-    if constexpr (NORM) {
-        if (a.residual) {
-            float o[8];
-            load8<T>((const T *)a.residual + row * a.H, i, a.H, true, o);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = rnd<T>(p[j] + o[j]);
+        for (int j = 0; j < 8; ++j) {
+            const float t = p[j] * inv;
+            if (__builtin_fabsf(t - ((t + kToInt) - kToInt)) > 0.5f - 0x1p-15f) u[j] = quant_exact(p[j], m, inv);
         }
-        float g[8];
-        load8<T>((const T *)a.gain, i, a.H, true, g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { r[j] = p[j]; p[j] = p[j] * g[j]; }
     }
+    uint2 o;
+    o.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u), __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), 0x05040100u);
+    o.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[7], u[6], 0x0c0c0400u), __builtin_amdgcn_perm(u[5], u[4], 0x0c0c0400u), 0x05040100u);
+    return o;
 }
 
-// One workgroup per row.  NV > 0: a thread keeps its NV groups of 8 columns in registers; NV = 0:
+// What a row holds and how it is read.
+enum RowMode {
+    kRowQuant = 0,       // the row itself, 16-byte loads
+    kRowQuantOdd = 1,    // the row itself, whatever its length and alignment
+    kRowNorm = 2,        // norm of x
+    kRowNormAdd = 3      // norm of x + residual
+};
+
+template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
+
+// 8 columns as they come from memory.  All loads of a row are issued before anything is computed (a branch between them
+// makes each wait for the one before: 183 us instead of 110 for the prefill case); groups past the row's end
+// re-read its last one and count as zeros.
+template <typename T, int MODE> struct RawCols {
+    typename Vec8<T>::type x, residual, gain;
+    __device__ __forceinline__ void load(const RowQuantArgs &a, int64_t row, int c, int nvec)
+    {
+        typedef typename Vec8<T>::type V8;
+        if constexpr (MODE == kRowQuantOdd) {
+            const T *src = (const T *)a.x + row * a.H;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = src[min(c * 8 + j, a.H - 1)];
+        } else {
+            const int64_t at = row * (a.H >> 3) + min(c, nvec - 1);
+            x = ((const V8 *)a.x)[at];
+            if constexpr (MODE == kRowNormAdd) residual = ((const V8 *)a.residual)[at];
+            if constexpr (MODE >= kRowNorm) gain = ((const V8 *)a.gain)[min(c, nvec - 1)];
+        }
+    }
+    // p: the values to quantise; returns the rounded sum (norm)
+    __device__ __forceinline__ typename Vec8<T>::type values(int c, int H, float *p) const
+    {
+        typename Vec8<T>::type r = x;
+        const bool in = c * 8 < H;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (MODE == kRowNormAdd) r[j] = (T)((float)x[j] + (float)residual[j]);
+            float v = (float)r[j];
+            if constexpr (MODE >= kRowNorm) v = v * (float)gain[j];
+            p[j] = (MODE == kRowQuantOdd ? c * 8 + j < H : in) ? v : 0.f;
+        }
+        if (MODE >= kRowNorm && !in) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = (T)0.f;
+        }
+        return r;
+    }
+};
+
+// WPR waves per row, RPB rows per workgroup.  NV > 0: a thread keeps its NV groups of 8 columns in registers; NV = 0:
 // rows too long for that are read twice (the second time mostly from L2).
-template <typename T, bool NORM, int NV, int THREADS>
-__global__ __launch_bounds__(THREADS) void row_quant_kernel(RowQuantArgs a)
+template <typename T, int MODE, int NV, int WPR, int RPB>
+__global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs a)
 {
-    constexpr int WAVES = THREADS / 64;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    static_assert(WPR == 1 || RPB == 1, "several rows per workgroup: one wave each");
+    typedef typename Vec8<T>::type V8;
+    constexpr bool NORM = MODE >= kRowNorm;
+    constexpr int THREADS = 64 * WPR;                      // of a row
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int tid = RPB > 1 ? lane : threadIdx.x;
     const int nvec = (a.H + 7) >> 3;
     constexpr int KEEP = NV ? NV : 1;
-    float p[KEEP][8], r[NORM ? KEEP : 1][8];
-    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
-        // The squares are summed in fp64: no overflow for any finite input, and no dependence of the result on
-        // the row's length (the kernel waits for memory: the two extra instructions per element are not seen).
+    for (int64_t row = RPB > 1 ? (int64_t)blockIdx.x * RPB + wave : blockIdx.x; row < a.n; row += (int64_t)gridDim.x * RPB) {
+        float p[KEEP][8];
+        V8 r[KEEP];
+        // Squares are summed in fp32 over 8 columns and in fp64 from there; a row whose squares do not fit fp32 (values
+        // beyond 2^63 in a bf16 row) is summed again in fp64 from the first, so that no finite row overflows.
         double ss = 0.0;
-        float m = 0.f;
-        auto take = [&](const float *pv, const float *rv) {
+        uint32_t mb = 0;                                   // max |p| as bits: NaN orders behind infinity
+        auto take = [&](const float *pv, const V8 &rv, bool wide) {
+            float q = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if constexpr (NORM) ss = __builtin_fma((double)rv[j], (double)rv[j], ss);
-                // a NaN must not be lost: max drops it, so it is carried as an infinity
-                const float v = __builtin_fabsf(pv[j]);
-                m = v <= __builtin_huge_valf() ? __builtin_fmaxf(m, v) : __builtin_huge_valf();
+                if constexpr (NORM) {
+                    const float f = (float)rv[j];
+                    if (wide) ss = __builtin_fma((double)f, (double)f, ss);
+                    else q = __builtin_fmaf(f, f, q);
+                }
+                mb = max(mb, __builtin_bit_cast(uint32_t, pv[j]) & 0x7fffffffu);
             }
+            if constexpr (NORM) ss += (double)q;
         };
-        if constexpr (NV > 0) {
+        auto take_row = [&](bool wide) {
+            if constexpr (NV > 0) {
 #pragma unroll
-            for (int u = 0; u < NV; ++u) {
-                const int c = u * THREADS + tid;
-                if (c < nvec) {
-                    row_values<T, NORM>(a, row, c * 8, p[u], NORM ? r[u] : nullptr);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) { p[u][j] = 0.f; if constexpr (NORM) r[u][j] = 0.f; }
+                for (int u = 0; u < NV; ++u) take(p[u], r[u], wide);
+            } else {
+                for (int c = tid; c < nvec; c += THREADS) {
+                    RawCols<T, MODE> raw;
+                    raw.load(a, row, c, nvec);
+                    r[0] = raw.values(c, a.H, p[0]);
+                    take(p[0], r[0], wide);
                 }
             }
 #pragma unroll
-            for (int u = 0; u < NV; ++u) take(p[u], NORM ? r[u] : nullptr);
-        } else {
-            for (int c = tid; c < nvec; c += THREADS) {
-                row_values<T, NORM>(a, row, c * 8, p[0], r[0]);
-                take(p[0], r[0]);
+            for (int d = 32; d >= 1; d >>= 1) {
+                if constexpr (NORM) ss += __shfl_xor(ss, d);
+                mb = max(mb, (uint32_t)__shfl_xor((int)mb, d));
+            }
+            if constexpr (WPR > 1) {
+                __shared__ double s_ss[WPR];
+                __shared__ uint32_t s_m[WPR];
+                if (lane == 0) { s_ss[wave] = ss; s_m[wave] = mb; }
+                __syncthreads();
+                ss = s_ss[0]; mb = s_m[0];
+#pragma unroll
+                for (int w = 1; w < WPR; ++w) { ss += s_ss[w]; mb = max(mb, s_m[w]); }
+                __syncthreads();                           // (the same LDS serves the next sums)
+            }
+        };
+        if constexpr (NV > 0) {
+            RawCols<T, MODE> raw[NV];
+#pragma unroll
+            for (int u = 0; u < NV; ++u) raw[u].load(a, row, u * THREADS + tid, nvec);
+#pragma unroll
+            for (int u = 0; u < NV; ++u) r[u] = raw[u].values(u * THREADS + tid, a.H, p[u]);
+        }
+        take_row(NORM && a.wide);
+        if constexpr (NORM) {
+            if (!a.wide && !(ss < __builtin_huge_val())) {  // (the same for every thread of the row)
+                ss = 0.0;
+                take_row(true);
             }
         }
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) {
-            if constexpr (NORM) ss += __shfl_xor(ss, d);
-            m = __builtin_fmaxf(m, __shfl_xor(m, d));
-        }
-        if constexpr (WAVES > 1) {
-            __shared__ double s_ss[WAVES];
-            __shared__ float s_m[WAVES];
-            if (lane == 0) { s_ss[wave] = ss; s_m[wave] = m; }
-            __syncthreads();
-            ss = s_ss[0]; m = s_m[0];
-#pragma unroll
-            for (int w = 1; w < WAVES; ++w) { ss += s_ss[w]; m = __builtin_fmaxf(m, s_m[w]); }
-        }
-        float rstd = 1.f;
+        const float m = __builtin_bit_cast(float, mb);
+        float rstd = 1.f, rlow = 0.f;
         if constexpr (NORM) {
-            // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40)
+            // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40), as two fp32
+            // values, so that a product with it rounds once
             const double ms = ss * a.inv_h + (double)a.eps;
             const double y0 = __builtin_amdgcn_rsq(ms);
-            rstd = (float)(y0 * (1.5 - 0.5 * ms * y0 * y0));      // NaN for a row with an infinity or NaN
+            const double y1 = y0 * (1.5 - 0.5 * ms * y0 * y0);    // NaN for a row with an infinity or NaN
+            rstd = (float)y1;
+            rlow = (float)(y1 - (double)rstd);
         }
         const bool finite = m < __builtin_huge_valf();
-        const float up = m < 0x1p-100f ? 0x1p64f : 1.f;
-        const float inv = m > 0.f && finite ? 127.f / (m * up) : 0.f;
         if (a.scale && tid == 0) a.scale[row] = !finite ? __builtin_nanf("") : NORM ? m * rstd / 127.f : m / 127.f;
+        // a row of tiny values is brought into the range of normal numbers (a power of two: exact) before 127 / m
+        const bool tiny = m < 0x1p-100f;
+        const float mq = tiny ? m * 0x1p64f : m;
+        const float inv = mq > 0.f && finite ? 127.f / mq : 0.f;
 
-        auto give = [&](int c, const float *pv, const float *rv) {
-            const int i = c * 8;
+        auto give = [&](int c, float *pv, const V8 &rv) {
             if constexpr (NORM) {
-                if (a.sum) store8<T>((T *)a.sum + row * a.H, i, rv);
+                const int64_t at = row * (a.H >> 3) + c;
+                if (a.sum) ((V8 *)a.sum)[at] = rv;
                 if (a.y) {
-                    float o[8];
+                    V8 o;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = as_fp32(pv[j] * rstd);
-                    store8<T>((T *)a.y + row * a.H, i, o);
+                    for (int j = 0; j < 8; ++j) o[j] = (T)as_fp32(__builtin_fmaf(pv[j], rstd, pv[j] * rlow));
+                    ((V8 *)a.y)[at] = o;
                 }
             }
             if (a.q) {
-                float k[8];
-                bool all = true;
+                if (tiny) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) all &= quant_fast(pv[j], inv, up, k[j]);
-                if (!all) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        float t;
-                        if (!quant_fast(pv[j], inv, up, t)) k[j] = quant_exact(pv[j], m, inv, up);
-                    }
+                    for (int j = 0; j < 8; ++j) pv[j] *= 0x1p64f;
                 }
-                uint32_t w[2] = {0, 0};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j >> 2] |= ((uint32_t)(int)k[j] & 0xffu) << (8 * (j & 3));
-                if (!finite) w[0] = w[1] = 0;
-                *(uint2 *)(a.q + row * a.q_stride + i) = uint2{w[0], w[1]};
+                uint2 o = quant8(pv, mq, inv);
+                if (!finite) o = uint2{0, 0};
+                *(uint2 *)(a.q + row * a.q_stride + c * 8) = o;
             }
         };
         if constexpr (NV > 0) {
 #pragma unroll
             for (int u = 0; u < NV; ++u) {
                 const int c = u * THREADS + tid;
-                if (c < nvec) give(c, p[u], NORM ? r[u] : nullptr);
+                if (c < nvec) give(c, p[u], r[u]);
             }
         } else {
             for (int c = tid; c < nvec; c += THREADS) {
-                row_values<T, NORM>(a, row, c * 8, p[0], r[0]);
+                RawCols<T, MODE> raw;
+                raw.load(a, row, c, nvec);
+                r[0] = raw.values(c, a.H, p[0]);
                 give(c, p[0], r[0]);
             }
         }
         // the padding of an int8 row that the products read in whole steps
         if (a.q)
             for (int i = nvec * 8 + tid * 8; i < a.q_stride; i += THREADS * 8) *(uint2 *)(a.q + row * a.q_stride + i) = uint2{0, 0};
-        if constexpr (WAVES > 1) __syncthreads();      // the next row's sums take the same LDS
     }
 }
 
 constexpr int64_t kMaxRowGroups = 1 << 21;     // a launch holds less than 2^32 threads
 
-template <typename T, bool NORM>
+// Launch shapes: one wave per row (no barrier, four rows per workgroup) as long as a lane's share is at most four groups
+// of columns and there are rows enough to fill the chip; else a workgroup per row, as wide as the row needs.
+// (MI355X, 65536 rows of 2048: 128 us with 256 threads per row, 85 with a wave.)
+template <typename T, int MODE>
 static void launch_rows(const RowQuantArgs &a, hipStream_t s)
 {
     const int nvec = (a.H + 7) / 8;
-    const dim3 grid((unsigned)(a.n < kMaxRowGroups ? a.n : kMaxRowGroups));
-#define EK_ROWS(NV, TH) hipLaunchKernelGGL((row_quant_kernel<T, NORM, NV, TH>), grid, dim3(TH), 0, s, a)
-    if (nvec <= 64) EK_ROWS(1, 64);
-    else if (nvec <= 256) EK_ROWS(1, 256);
-    else if (nvec <= 512) EK_ROWS(2, 256);
-    else if (nvec <= 1024) EK_ROWS(4, 256);
-    else if (nvec <= 4096) EK_ROWS(4, 1024);
-    else EK_ROWS(0, 1024);
+#define EK_ROWS(NV, WPR, RPB)                                                                                             \
+    hipLaunchKernelGGL((row_quant_kernel<T, MODE, NV, WPR, RPB>),                                                          \
+                       dim3((unsigned)std::min<int64_t>((a.n + RPB - 1) / RPB, kMaxRowGroups)), dim3(64 * WPR * RPB), 0, s, a)
+    if constexpr (MODE == kRowQuantOdd) {
+        if (nvec <= 256) EK_ROWS(1, 4, 1);
+        else EK_ROWS(0, 16, 1);
+    } else {
+        if (nvec <= 64) EK_ROWS(1, 1, 4);
+        else if (nvec <= 256 && a.n >= 2048) { if (nvec <= 128) EK_ROWS(2, 1, 4); else EK_ROWS(4, 1, 4); }
+        else if (nvec <= 256) EK_ROWS(1, 4, 1);
+        else if (nvec <= 512) EK_ROWS(2, 4, 1);
+        else if (nvec <= 1024) { if (a.n < 512) EK_ROWS(1, 16, 1); else EK_ROWS(4, 4, 1); }
+        else if (nvec <= 4096) EK_ROWS(4, 16, 1);
+        else EK_ROWS(0, 16, 1);
+    }
 #undef EK_ROWS
+}
+
+template <typename T> static void launch_mode(const RowQuantArgs &a, bool norm, hipStream_t s)
+{
+    if (norm) a.residual ? launch_rows<T, kRowNormAdd>(a, s) : launch_rows<T, kRowNorm>(a, s);
+    else a.vec ? launch_rows<T, kRowQuant>(a, s) : launch_rows<T, kRowQuantOdd>(a, s);
 }
 
 hipError_t launch_row_quant(const RowQuantArgs &a, int act, bool norm, hipStream_t s)
 {
     if (a.n <= 0) return hipSuccess;
-    if (act == 0) norm ? launch_rows<__bf16, true>(a, s) : launch_rows<__bf16, false>(a, s);
-    else norm ? launch_rows<_Float16, true>(a, s) : launch_rows<_Float16, false>(a, s);
+    if (act == 0) launch_mode<__bf16>(a, norm, s);
+    else launch_mode<_Float16>(a, norm, s);
     return hipGetLastError();
 }
 

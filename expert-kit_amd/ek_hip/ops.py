@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _capi as C
-from .backend import _DT, _NO_CTX, _alloc_on, _desc, _mem, _stream_ptr
+from .backend import _DT, _alloc_on, _desc, _mem, _stream_ptr
 
 
 def _check_device(t: torch.Tensor, device_id: int) -> None:
@@ -41,6 +41,7 @@ class HipNorm:
         if gain.dim() != 1 or gain.dtype not in (torch.bfloat16, torch.float16):
             raise C.EKError(C.EK_INVALID_INPUT, f"gain must be a bf16 or fp16 vector (got {tuple(gain.shape)} {gain.dtype})")
         self._lib = C.load()
+        self._forward = self._lib.ek_norm_forward
         self.hidden, self.dtype, self.device_id = gain.numel(), gain.dtype, device_id
         _check_device(gain, device_id)
         gain = gain.contiguous()
@@ -52,26 +53,32 @@ class HipNorm:
                 stream=None, out: Optional[NormOut] = None) -> NormOut:
         """x, residual [n, H] -> NormOut.  norm / quantize: which outputs to make (the sum is made when there is a
         residual).  out: the tensors to write, in place of the three switches; its sum may be x or residual."""
-        H, n = self.hidden, x.shape[0]
+        H, dev = self.hidden, x.device
         if x.dim() != 2 or x.shape[1] != H or x.dtype != self.dtype:
             raise C.EKError(C.EK_INVALID_INPUT, f"x must be [n, {H}] {self.dtype} (got {tuple(x.shape)} {x.dtype})")
-        _check_device(x, self.device_id)
-        if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        on_gpu = dev.type == "cuda"
+        if on_gpu and dev.index != self.device_id:
+            _check_device(x, self.device_id)
+        if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev):
             raise C.EKError(C.EK_INVALID_INPUT, "residual must be like x")
-        with _alloc_on(stream) if out is None or not x.is_contiguous() or (residual is not None and not residual.is_contiguous()) else _NO_CTX:
-            x = x.contiguous()
-            residual = residual.contiguous() if residual is not None else None
-            if out is None:
-                out = NormOut(torch.empty_like(x) if residual is not None else None, torch.empty_like(x) if norm else None,
-                              torch.empty(n, H, dtype=torch.int8, device=x.device) if quantize else None,
-                              torch.empty(n, dtype=torch.float32, device=x.device) if quantize else None)
-            else:
-                for t, name, shape, dt in ((out.sum, "sum", (n, H), x.dtype), (out.y, "y", (n, H), x.dtype),
-                                           (out.q, "q", (n, H), torch.int8), (out.scale, "scale", (n,), torch.float32)):
-                    if t is not None and (tuple(t.shape) != shape or t.dtype != dt or t.device != x.device or not t.is_contiguous()):
-                        raise C.EKError(C.EK_INVALID_INPUT, f"out.{name} must be a contiguous {shape} {dt} tensor beside x")
-        C.check(self._lib.ek_norm_forward(self._h, _addr(x), _addr(residual), n, _addr(out.sum), _addr(out.y), _addr(out.q),
-                                          _addr(out.scale), _mem(x), _stream_ptr(stream)))
+        n = x.shape[0]
+        if out is None or not x.is_contiguous() or (residual is not None and not residual.is_contiguous()):
+            with _alloc_on(stream):
+                x = x.contiguous()
+                residual = residual.contiguous() if residual is not None else None
+                if out is None:
+                    out = NormOut(torch.empty_like(x) if residual is not None else None, torch.empty_like(x) if norm else None,
+                                  torch.empty(n, H, dtype=torch.int8, device=dev) if quantize else None,
+                                  torch.empty(n, dtype=torch.float32, device=dev) if quantize else None)
+        total, y, q, scale = out
+        for t, name, shape, dt in ((total, "sum", (n, H), x.dtype), (y, "y", (n, H), x.dtype), (q, "q", (n, H), torch.int8),
+                                   (scale, "scale", (n,), torch.float32)):
+            if t is not None and (t.shape != shape or t.dtype != dt or t.device != dev or not t.is_contiguous()):
+                raise C.EKError(C.EK_INVALID_INPUT, f"out.{name} must be a contiguous {shape} {dt} tensor beside x")
+        status = self._forward(self._h, x.data_ptr(), _addr(residual), n, _addr(total), _addr(y), _addr(q), _addr(scale),
+                               C.EK_DEVICE if on_gpu else C.EK_HOST, _stream_ptr(stream))
+        if status:
+            C.check(status)
         return out
 
     def shape(self):
@@ -128,12 +135,14 @@ class HipLinear:
         if out is not None and (tuple(out.shape) != (n, self.out_features) or out.dtype != self.act_dtype or out.device != x.device
                                 or not out.is_contiguous()):
             raise C.EKError(C.EK_INVALID_INPUT, "out must be a contiguous [n, N] tensor of the activation dtype beside x")
-        with _alloc_on(stream) if out is None or not x.is_contiguous() or (scale is not None and not scale.is_contiguous()) else _NO_CTX:
-            x = x.contiguous()
-            scale = scale.contiguous() if scale is not None else None
-            y = out if out is not None else torch.empty(n, self.out_features, dtype=self.act_dtype, device=x.device)
-        C.check(self._lib.ek_linear_forward(self._h, _addr(x), _addr(scale), n, _addr(y), _mem(x), _stream_ptr(stream)))
-        return y
+        if out is None or not x.is_contiguous() or (scale is not None and not scale.is_contiguous()):
+            with _alloc_on(stream):
+                x = x.contiguous()
+                scale = scale.contiguous() if scale is not None else None
+                if out is None:
+                    out = torch.empty(n, self.out_features, dtype=self.act_dtype, device=x.device)
+        C.check(self._lib.ek_linear_forward(self._h, _addr(x), _addr(scale), n, _addr(out), _mem(x), _stream_ptr(stream)))
+        return out
 
     def shape(self):
         k, n = ctypes.c_int64(), ctypes.c_int64()

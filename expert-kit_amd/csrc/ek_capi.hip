@@ -1243,7 +1243,8 @@ bool pair_direct_fits(const ek_layer *L, int64_t T)
 {
     const int64_t P = T * L->cfg.top_k;
     const SharedCut sc = shared_cut(L, T);          // a shared expert of the routed experts' shape is one more wave
-    return !L->act8 && P > 0 && P <= kPairDirectPairs && L->cfg.top_k <= ek::kPairDirectMaxK && (!sc.shared || !sc.own);
+    if (L->act8 && !ek::q8_pairs_fit(P, L->cfg.top_k, L->cfg.hidden, L->cfg.inter)) return false;
+    return P > 0 && P <= kPairDirectPairs && L->cfg.top_k <= ek::kPairDirectMaxK && (!sc.shared || !sc.own);
 }
 
 // want_tables: the caller reads the call's routing tables or packed expert outputs afterwards.
@@ -1265,6 +1266,24 @@ ek_status enqueue_forward(ek_layer *L, const Workspace &W, const void *x, const 
     // A decode call of one or two tokens: its few pairs run as one-row items straight from the ids,
     // and stage 2 adds a token's pairs itself: two kernels instead of four (no pack, no combine;
     // DeepSeek-V3 int8 layer on MI355X, 1 / 2 tokens: see kPairDirectPairs).  Same bits.
+    if (!routed && !want_tables && L->act8 && pair_direct_fits(L, T)) {
+        ek::Q8Args up{};
+        up.x = x_scale ? (const uint8_t *)x : nullptr; up.x_scale = x_scale; up.slabs = L->d_slabs; up.out = W.h; up.out_stride = L->cfg.inter;
+        up.N = (int32_t)L->cfg.inter; up.NT = (int32_t)(L->cfg.inter / 16); up.Kdim = (int32_t)H;
+        ek::Q8Args down = up;
+        down.x = nullptr; down.x_scale = nullptr; down.out = nullptr; down.out_stride = H;
+        down.N = (int32_t)H; down.NT = (int32_t)(H / 16); down.Kdim = (int32_t)L->cfg.inter;
+        ek::PairArgs pa{};
+        pa.ids = ids; pa.P = (int32_t)P; pa.K = K; pa.n_experts = E; pa.shared = shared_cut(L, T).shared ? 1 : 0;
+        pa.x16 = x_scale ? nullptr : x; pa.h = W.h; pa.w = w; pa.w_f32 = w_f32; pa.y = y;
+        pa.err = W.err; pa.activation = L->d_activation; pa.tile_items_host = L->d_tile_items;
+        for (int i = 1; i <= 2 && ev; ++i) EK_HIP(hipEventRecord(ev[i], s));     // (both kernels count as the down phase)
+        EK_HIP(ek::launch_pairs_q8(up, down, pa, L->act, s));
+        if (ev) EK_HIP(hipEventRecord(ev[3], s));
+        if (before_combine) EK_TRY((*before_combine)());
+        if (ev) EK_HIP(hipEventRecord(ev[4], s));
+        return EK_OK;
+    }
     if (!routed && !want_tables && pair_direct_fits(L, T)) {
         ek::FfnArgs a1;
         a1.x = x; a1.x_stride = H; a1.rows = nullptr; a1.slabs = L->d_slabs; a1.out = W.h; a1.out_stride = L->cfg.inter;

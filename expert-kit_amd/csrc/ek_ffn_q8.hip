@@ -9,6 +9,7 @@
 // v_mfma_i32_16x16x64_i8 as it is, but for the offset-binary storage: q = u ^ 0x80.
 #include "ek_internal.h"
 #include "ek_mfma.h"
+#include "ek_quant.h"
 
 #include <type_traits>
 
@@ -173,6 +174,198 @@ __global__ __launch_bounds__(64 * kQ8Slices) void q8_stream_kernel(Q8Args a, int
     }
 }
 
+
+// ---- pair-direct calls: a few (token, expert) pairs, two kernels ------------------------------------------
+//
+// Every pair is a one-row item taken straight from the ids, as launch_ffn_pairs does for 16-bit activations.
+// Stage 1: blockIdx.y is the pair; the eight waves take an eighth of the contraction each.  With 16-bit rows of x the
+// workgroup quantises its row first (into LDS).  Stage 2: blockIdx.y is the token, wave k takes its k-th pair: it
+// quantises the pair's row of h into LDS, walks the whole contraction, and the first wave adds the
+// rounded outputs with the gate weights in k order, as the combine kernel does.  The integer sums are exact and the codes
+// are functions of their row, so the results are those of the call through pack and combine, bit for bit.
+
+// What the pack kernel would have stored of the call's bookkeeping; one wave.
+__device__ __forceinline__ void pair_bookkeeping(const PairArgs &pa, const ExpertSlab *slabs, int lane)
+{
+    const int32_t id = lane < pa.P ? pa.ids[lane] : 0;
+    const bool bad = lane < pa.P && (uint32_t)id >= (uint32_t)pa.n_experts, ok = lane < pa.P && !bad;
+    const bool unloaded = ok && slabs[id].upgate == nullptr;
+    const uint64_t any_bad = __ballot(bad), any_unloaded = __ballot(unloaded);
+    if (ok && pa.activation) atomicAdd((unsigned long long *)&pa.activation[id], 1ull);
+    if (lane == 0) {
+        pa.err[0] = (any_bad ? 1 : 0) | (any_unloaded ? 2 : 0);
+        if (pa.tile_items_host) *pa.tile_items_host = 0;
+    }
+}
+
+// The codes of one row of n 16-bit values (n a multiple of 64) by the THREADS lanes that hold it, into LDS; returns the
+// scale.  red: one word per wave.
+template <typename T, int WAVES>
+__device__ __forceinline__ float q8_row_to_lds(const T *row, int n, uint8_t *codes, uint32_t *red)
+{
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = WAVES == 1 ? lane : threadIdx.x;
+    uint32_t mb = 0;
+    for (int c = tid; c < n / 8; c += 64 * WAVES) {
+        const V8 v = *(const V8 *)(row + c * 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mb = max(mb, __builtin_bit_cast(uint32_t, (float)v[j]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) mb = max(mb, (uint32_t)__shfl_xor((int)mb, d));
+    if constexpr (WAVES > 1) {
+        if (lane == 0) red[wave] = mb;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) mb = max(mb, red[w]);
+    }
+    const QuantRow q(__builtin_bit_cast(float, mb));
+    for (int c = tid; c < n / 8; c += 64 * WAVES) {
+        const V8 v = *(const V8 *)(row + c * 8);
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
+        *(uint2 *)(codes + c * 8) = q.codes(f);
+    }
+    return q.scale();
+}
+
+template <typename T>
+__global__ __launch_bounds__(64 * kQ8Slices) void q8_pairs_up_kernel(Q8Args a, PairArgs pa)
+{
+    extern __shared__ __align__(16) uint8_t q8_lds[];            // 16-bit rows: the codes of this pair's row
+    __shared__ uint32_t red_m[kQ8Slices];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && wave == 0) pair_bookkeeping(pa, a.slabs, lane);
+    const int pair = blockIdx.y;
+    const bool shared_row = pair >= pa.P;
+    const int e = shared_row ? pa.n_experts : pa.ids[pair];
+    if (!shared_row && (uint32_t)e >= (uint32_t)pa.n_experts) return;
+    const ExpertSlab slab = a.slabs[e];
+    if (slab.upgate == nullptr) return;
+    const int64_t row = shared_row ? pair - pa.P : pair / pa.K;
+    const int KT = a.Kdim >> 6, nt = blockIdx.x;
+    const int kbeg = KT * wave / kQ8Slices, kend = KT * (wave + 1) / kQ8Slices;
+    const uint8_t *wp = slab.upgate + (int64_t)nt * KT * (2 * kChunkBytes) + lane * 16;
+    constexpr int D = 4;
+    uint4 wq[D][2];
+    auto fetch = [&](int d, int kt) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) wq[d][m] = ldg16_once(wp + (int64_t)(kt * 2 + m) * kChunkBytes);
+    };
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        if (kbeg + d < kend) fetch(d, kbeg + d);
+    float xs;
+    if (pa.x16) xs = q8_row_to_lds<T, kQ8Slices>((const T *)pa.x16 + row * a.Kdim, a.Kdim, q8_lds, red_m);
+    else xs = a.x_scale[row];
+    if (pa.x16) __syncthreads();
+    const uint8_t *xg = a.x + row * a.Kdim + g * 16, *xl = q8_lds + g * 16;
+    i32x4 acc[2] = {i32x4{0, 0, 0, 0}, i32x4{0, 0, 0, 0}};
+    for (int kt0 = kbeg; kt0 < kend; kt0 += D) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int kt = kt0 + d;
+            if (kt >= kend) break;
+            const i32x4 x = pa.x16 ? *(const i32x4 *)(xl + kt * 64) : __builtin_bit_cast(i32x4, ldg16(xg + kt * 64));
+#pragma unroll
+            for (int m = 0; m < 2; ++m) acc[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(signed8(wq[d][m]), x, acc[m], 0, 0, 0);
+            if (kt + D < kend) fetch(d, kt + D);
+        }
+    }
+    // every column of the result is the row: lanes j = 0 keep it
+    __shared__ i32x4 red[kQ8Slices][2][4];
+    if (j == 0) { red[wave][0][g] = acc[0]; red[wave][1][g] = acc[1]; }
+    __syncthreads();
+    if (threadIdx.x >= 16) return;
+    const int ch = nt * 16 + threadIdx.x;
+    int up = 0, gate = 0;
+#pragma unroll
+    for (int w = 0; w < kQ8Slices; ++w) {
+        up += red[w][0][threadIdx.x >> 2][threadIdx.x & 3];
+        gate += red[w][1][threadIdx.x >> 2][threadIdx.x & 3];
+    }
+    ((T *)a.out)[(int64_t)pair * a.out_stride + ch] =
+        swiglu_rounded<T>(as_fp32((float)up * (xs * slab.s_up[ch])), as_fp32((float)gate * (xs * slab.s_gate[ch])));
+}
+
+constexpr int kPairTiles = 2;            // channel tiles of a stage-2 workgroup
+template <typename T>
+__global__ __launch_bounds__(64 * (kPairDirectMaxK + 1)) void q8_pairs_down_kernel(Q8Args a, PairArgs pa)
+{
+    extern __shared__ __align__(16) uint8_t q8_lds[];            // [waves][Kdim]: the codes of the pairs' rows of h
+    __shared__ float prod[kPairDirectMaxK + 1][kPairTiles * 16];
+    __shared__ int32_t valid[kPairDirectMaxK + 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+    const int64_t t = blockIdx.y;
+    const bool shared_row = wave == pa.K;
+    const int64_t pair = shared_row ? pa.P + t : t * pa.K + wave;
+    int e = shared_row ? pa.n_experts : pa.ids[pair];
+    bool live = shared_row || (uint32_t)e < (uint32_t)pa.n_experts;
+    const ExpertSlab slab = a.slabs[live ? e : 0];
+    live = live && slab.down != nullptr;
+    const int nt0 = blockIdx.x * kPairTiles;
+    if (lane == 0) valid[wave] = live;
+    if (live) {
+        const int KT = a.Kdim >> 6;
+        const uint8_t *wp[kPairTiles];
+#pragma unroll
+        for (int gi = 0; gi < kPairTiles; ++gi) wp[gi] = slab.down + (int64_t)min(nt0 + gi, a.NT - 1) * KT * kChunkBytes + lane * 16;
+        constexpr int D = 4;
+        uint4 wq[D][kPairTiles];
+        auto fetch = [&](int d, int kt) {
+#pragma unroll
+            for (int gi = 0; gi < kPairTiles; ++gi) wq[d][gi] = ldg16_once(wp[gi] + (int64_t)kt * kChunkBytes);
+        };
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+            if (d < KT) fetch(d, d);
+        uint8_t *codes = q8_lds + (int64_t)wave * a.Kdim;
+        const float hs = q8_row_to_lds<T, 1>((const T *)pa.h + pair * a.Kdim, a.Kdim, codes, nullptr);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        i32x4 acc[kPairTiles];
+#pragma unroll
+        for (int gi = 0; gi < kPairTiles; ++gi) acc[gi] = i32x4{0, 0, 0, 0};
+        for (int kt0 = 0; kt0 < KT; kt0 += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                const int kt = kt0 + d;
+                if (kt >= KT) break;
+                const i32x4 x = *(const i32x4 *)(codes + kt * 64 + g * 16);
+#pragma unroll
+                for (int gi = 0; gi < kPairTiles; ++gi)
+                    acc[gi] = __builtin_amdgcn_mfma_i32_16x16x64_i8(signed8(wq[d][gi]), x, acc[gi], 0, 0, 0);
+                if (kt + D < KT) fetch(d, kt + D);
+            }
+        }
+        if (j == 0) {
+            const int64_t wi = shared_row ? 0 : pair;
+            const float gw = pa.w_f32 ? ((const float *)pa.w)[wi] : (float)((const T *)pa.w)[wi];
+#pragma unroll
+            for (int gi = 0; gi < kPairTiles; ++gi)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int ch = min((nt0 + gi) * 16 + 4 * g + r, a.NT * 16 - 1);
+                    float v = (float)(T)as_fp32((float)acc[gi][r] * (hs * slab.s_down[ch]));
+                    if (!shared_row) {
+                        v = as_fp32(gw * v);
+                        if (!pa.w_f32) v = (float)(T)v;
+                    }
+                    prod[wave][gi * 16 + 4 * g + r] = v;
+                }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= kPairTiles * 16 || nt0 * 16 + (int)threadIdx.x >= a.N) return;
+    float sum = 0.f;
+    for (int k = 0; k < pa.K; ++k)
+        if (valid[k]) sum = sum + prod[k][threadIdx.x];
+    T o = (T)sum;
+    if (pa.shared && valid[pa.K]) o = (T)((float)o + prod[pa.K][threadIdx.x]);       // after the sum's rounding
+    ((T *)pa.y)[t * a.out_stride + nt0 * 16 + threadIdx.x] = o;
+}
 
 // ---- tile kernel: items of up to 256 rows -------------------------------------------------------------
 //
@@ -524,6 +717,23 @@ hipError_t launch_dense_q8(const Q8Args &a, int act, hipStream_t s)
 {
     if (a.dense_rows <= 0) return hipSuccess;
     return act == 0 ? launch_dense_t<__bf16>(a, s) : launch_dense_t<_Float16>(a, s);
+}
+
+template <typename T> static hipError_t launch_pairs_t(const Q8Args &up, const Q8Args &down, const PairArgs &pa, hipStream_t s)
+{
+    const int T_ = pa.P / pa.K, rows = pa.P + (pa.shared ? T_ : 0);
+    hipLaunchKernelGGL(q8_pairs_up_kernel<T>, dim3((unsigned)up.NT, (unsigned)rows), dim3(64 * kQ8Slices), pa.x16 ? up.Kdim : 0, s, up, pa);
+    const int waves = pa.K + (pa.shared ? 1 : 0);
+    hipLaunchKernelGGL(q8_pairs_down_kernel<T>, dim3((unsigned)((down.NT + kPairTiles - 1) / kPairTiles), (unsigned)T_), dim3(64 * waves),
+                       (size_t)waves * down.Kdim, s, down, pa);
+    return hipGetLastError();
+}
+
+hipError_t launch_pairs_q8(const Q8Args &up, const Q8Args &down, const PairArgs &pa, int act, hipStream_t s)
+{
+    if (pa.P <= 0) return hipSuccess;
+    if (!q8_pairs_fit(pa.P, pa.K, up.Kdim, down.Kdim)) return hipErrorInvalidValue;
+    return act == 0 ? launch_pairs_t<__bf16>(up, down, pa, s) : launch_pairs_t<_Float16>(up, down, pa, s);
 }
 
 }  // namespace ek

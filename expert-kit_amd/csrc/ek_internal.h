@@ -265,6 +265,27 @@ struct Q8Args {
 // wide: the streaming list holds items of up to kWideRows rows
 hipError_t launch_ffn_q8(const Q8Args &a, int stage, int act, const int64_t max_items[kNumLists], bool wide, hipStream_t s);
 hipError_t launch_dense_q8(const Q8Args &a, int act, hipStream_t s);
+// A decode call of a few pairs without pack, quantisation and combine kernels (as launch_ffn_pairs): up (a.x with
+// x_scale, or pa.x16; out = h rows in pair order) and down (out_stride = N) stage arguments.
+struct PairArgs {
+    const int32_t *ids;       // [P]
+    int32_t P, K, n_experts;
+    int32_t shared;           // 1: every token also runs expert n_experts, rows P .. P + T - 1 of h
+    const void *x16;          // 16-bit rows of x, or nullptr: 8-bit ones in the stage's arguments
+    const void *h;            // stage 1's output
+    const void *w;            // [P] gate weights
+    int32_t w_f32;
+    void *y;                  // [T, N]
+    int32_t *err;             // the call's bookkeeping, as the pack kernel would store it
+    uint64_t *activation;
+    int32_t *tile_items_host;
+};
+// LDS holds a token's rows of h as codes (and stage 1's row of x)
+inline bool q8_pairs_fit(int64_t P, int64_t K, int64_t hidden, int64_t inter)
+{
+    return P > 0 && P <= kPairDirectMax && K <= kPairDirectMaxK && P % K == 0 && (kPairDirectMaxK + 1) * inter <= 60 * 1024 && hidden <= 60 * 1024;
+}
+hipError_t launch_pairs_q8(const Q8Args &up, const Q8Args &down, const PairArgs &pa, int act, hipStream_t s);
 
 // ---- combine ----------------------------------------------------------------
 struct CombineArgs {

@@ -13,50 +13,11 @@
 // of squares and its maximum together and writes everything from registers.
 #include "ek_internal.h"
 #include "ek_mfma.h"
+#include "ek_quant.h"
 
 #include <algorithm>
 
 namespace ek {
-
-// rint(127 p / m) for |p| <= m, as inv = 127 / m times p.  The fp32 product t is within 2^-22 relative of the real
-// value, so it decides unless it lies within 2^-15 of a half-integer; there 254 |p| is compared with the
-// odd multiple of m that the half-integer stands for, both exact in fp64 (24 + 8 bits).
-//
-// Adding 1.5 * 2^23 rounds t to the nearest integer, ties to even, and leaves it in the low byte of the sum as the
-// two's complement code.
-constexpr float kToInt = 12582912.f;
-__device__ __forceinline__ uint32_t quant_exact(float p, float m, float inv)
-{
-    const float a = __builtin_fabsf(p);
-    const float f = __builtin_floorf(a * inv);
-    const double lhs = 254.0 * (double)a, rhs = (2.0 * (double)f + 1.0) * (double)m;
-    const bool odd = ((int)f & 1) != 0;
-    const int k = (int)f + (lhs > rhs || (lhs == rhs && odd) ? 1 : 0);
-    return (uint32_t)(p < 0.f ? -k : k);
-}
-// 8 codes as bytes
-__device__ __forceinline__ uint2 quant8(const float *p, float m, float inv)
-{
-    uint32_t u[8];
-    float worst = 0.f;               // distance to the nearest integer: 1/2 on a border
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float t = p[j] * inv, s = t + kToInt;
-        worst = __builtin_fmaxf(worst, __builtin_fabsf(t - (s - kToInt)));
-        u[j] = __builtin_bit_cast(uint32_t, s);
-    }
-    if (worst > 0.5f - 0x1p-15f) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float t = p[j] * inv;
-            if (__builtin_fabsf(t - ((t + kToInt) - kToInt)) > 0.5f - 0x1p-15f) u[j] = quant_exact(p[j], m, inv);
-        }
-    }
-    uint2 o;
-    o.x = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[3], u[2], 0x0c0c0400u), __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), 0x05040100u);
-    o.y = __builtin_amdgcn_perm(__builtin_amdgcn_perm(u[7], u[6], 0x0c0c0400u), __builtin_amdgcn_perm(u[5], u[4], 0x0c0c0400u), 0x05040100u);
-    return o;
-}
 
 // What a row holds and how it is read.
 enum RowMode {
@@ -193,12 +154,8 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
             rstd = (float)y1;
             rlow = (float)(y1 - (double)rstd);
         }
-        const bool finite = m < __builtin_huge_valf();
-        if (a.scale && tid == 0) a.scale[row] = !finite ? __builtin_nanf("") : NORM ? m * rstd / 127.f : m / 127.f;
-        // a row of tiny values is brought into the range of normal numbers (a power of two: exact) before 127 / m
-        const bool tiny = m < 0x1p-100f;
-        const float mq = tiny ? m * 0x1p64f : m;
-        const float inv = mq > 0.f && finite ? 127.f / mq : 0.f;
+        const QuantRow quant(m);
+        if (a.scale && tid == 0) a.scale[row] = NORM ? quant.scale_of(m * rstd) : quant.scale();
 
         auto give = [&](int c, float *pv, const V8 &rv) {
             if constexpr (NORM) {
@@ -212,12 +169,7 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
                 }
             }
             if (a.q) {
-                if (tiny) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) pv[j] *= 0x1p64f;
-                }
-                uint2 o = quant8(pv, mq, inv);
-                if (!finite) o = uint2{0, 0};
+                const uint2 o = quant.codes(pv);
                 *(uint2 *)(a.q + row * a.q_stride + c * 8) = o;
             }
         };
@@ -245,7 +197,7 @@ constexpr int64_t kMaxRowGroups = 1 << 21;     // a launch holds less than 2^32 
 
 // Launch shapes: one wave per row (no barrier, four rows per workgroup) as long as a lane's share is at most four groups
 // of columns and there are rows enough to fill the chip; else a workgroup per row, as wide as the row needs.
-// (MI355X, 65536 rows of 2048: 128 us with 256 threads per row, 85 with a wave.)
+// (MI355X, 65536 rows of 2048: 98 us with 256 threads per row, 69 with a wave.)
 template <typename T, int MODE>
 static void launch_rows(const RowQuantArgs &a, hipStream_t s)
 {
@@ -262,7 +214,7 @@ static void launch_rows(const RowQuantArgs &a, hipStream_t s)
         else if (nvec <= 256) EK_ROWS(1, 4, 1);
         else if (nvec <= 512) EK_ROWS(2, 4, 1);
         else if (nvec <= 1024) { if (a.n < 512) EK_ROWS(1, 16, 1); else EK_ROWS(4, 4, 1); }
-        else if (nvec <= 4096) EK_ROWS(4, 16, 1);
+        else if (nvec <= 2048) EK_ROWS(2, 16, 1);
         else EK_ROWS(0, 16, 1);
     }
 #undef EK_ROWS

@@ -898,7 +898,7 @@ ek_status copy_route_out(ek_layer *L, const Workspace &W, const ek_route_out *r,
 }
 
 // The work lists of a layer call of P pairs (the same cut for pack, an appended shared segment and the launches).
-int one_class_of(const ek_layer *L, int64_t P) { return L->act8 ? ek::q8_one_class(P, L->cfg.n_experts) : 0; }
+int one_class_of(const ek_layer *L, int64_t P) { return L->act8 ? ek::q8_one_class(P, L->cfg.n_experts, L->cfg.hidden, L->cfg.inter) : 0; }
 ek::WorkLists lists_of(const ek_layer *L, const Workspace &W, int64_t P)
 {
     ek::WorkLists l = W.lists;
@@ -1042,7 +1042,7 @@ ek_status enqueue_ffn(ek_layer *L, const Workspace &W, const void *x, const int3
             const int64_t wcap[ek::kNumLists] = {wide_items, 0, 0, 0};
             return enqueue_ffn_q8(L, W, (const uint8_t *)x, x_scale, rows, out, h_rows, wcap, true, 0, s, ev);
         }
-        return enqueue_ffn_q8(L, W, (const uint8_t *)x, x_scale, rows, out, h_rows, cap, false, shared_wide, s, ev);
+        return enqueue_ffn_q8(L, W, (const uint8_t *)x, x_scale, rows, out, h_rows, cap, one_class == 3, shared_wide, s, ev);
     }
     if (wide_items > 0) {
         EK_HIP(ek::launch_ffn_stream(a1, 1, L->act, L->wmode, wide_items, true, false, s));
@@ -1150,11 +1150,19 @@ SharedCut shared_cut(const ek_layer *L, int64_t T)
 
 // The routing half of a layer call on stream s: pack, and the shared expert's segment appended to
 // its work lists.  It reads nothing but the ids, so a chain may run it ahead of the layer's turn.
-ek_status enqueue_route(ek_layer *L, const Workspace &W, const int32_t *ids, int64_t T, hipStream_t s)
+// x (EK_CFG_ACT8, or nullptr): 16-bit rows that may be quantised on the way; *quantised says whether they were.
+ek_status enqueue_route(ek_layer *L, const Workspace &W, const int32_t *ids, int64_t T, hipStream_t s, const void *x = nullptr,
+                        bool *quantised = nullptr)
 {
     const int E = L->cfg.n_experts;
     const int64_t P = T * L->cfg.top_k;
-    ek::launch_pack(pack_args(L, W, ids, P, true), s);
+    ek::PackArgs pack = pack_args(L, W, ids, P, true);
+    if (x) {
+        pack.quant_x = x; pack.quant_T = T; pack.quant_H = (int32_t)L->cfg.hidden; pack.quant_act = L->act;
+        pack.quant_q = W.xq; pack.quant_scale = W.xq_scale;
+    }
+    const bool done = ek::launch_pack(pack, s);
+    if (quantised) *quantised = done;
     const SharedCut sc = shared_cut(L, T);
     if (sc.own) {
         ek::launch_segment_lists(W.slists, E, (int32_t)P, (int32_t)T, W.row_token, sc.streamed ? 1 : sc.wide ? 2 : 0, s);
@@ -1304,7 +1312,8 @@ ek_status enqueue_forward(ek_layer *L, const Workspace &W, const void *x, const 
         if (ev) EK_HIP(hipEventRecord(ev[4], s));
         return EK_OK;
     }
-    if (!routed) EK_TRY(enqueue_route(L, W, ids, T, s));
+    bool quantised = false;
+    if (!routed) EK_TRY(enqueue_route(L, W, ids, T, s, L->act8 && !x_scale ? x : nullptr, &quantised));
     // the shared expert is one more segment: every token once, rows P .. P+T-1 of the packed buffers.
     // As tiles a decode-sized shared segment would occupy 8 to 14 CUs for the length of the whole
     // contraction.  Up to kSharedStreamRows tokens it is cut into 16-row streaming items
@@ -1315,7 +1324,7 @@ ek_status enqueue_forward(ek_layer *L, const Workspace &W, const void *x, const 
     const bool shared = sc.shared, shared_streamed = sc.streamed && !sc.own, shared_wide = sc.wide && !sc.own;
     if (ev) EK_HIP(hipEventRecord(ev[1], s));
     if (L->act8 && !x_scale && P > 0) {
-        EK_TRY(enqueue_quant(L, x, T, H, W.xq, W.xq_scale, s));
+        if (!quantised) EK_TRY(enqueue_quant(L, x, T, H, W.xq, W.xq_scale, s));
         x = W.xq;
         x_scale = W.xq_scale;
     }

@@ -61,7 +61,7 @@ struct WorkLists {
     int32_t *count;              // [kNumLists]
     // 1: a segment of more than 16 rows goes into the 128-row list whole, in as few items of at most kQ8Rows rows as
     // hold it, cut evenly in blocks of 32 rows (layers on 8-bit activations, whose tile kernel takes 1 .. kQ8Rows rows);
-    // 2: every segment does, however short
+    // 2: every segment does, however short; 3: every segment into the streaming list, in items of up to kWideRows rows
     int32_t one_class = 0;
 };
 constexpr int kWideRows = 64;
@@ -85,6 +85,7 @@ inline bool wide_cut_pays(int64_t tile_items, int64_t rows, int64_t hidden, int6
 }
 inline int64_t list_capacity(int list, int64_t P, int64_t E, int one_class = 0)
 {
+    if (one_class == 3) return list == kListStream ? P / kWideRows + (P < E ? P : E) : 0;
     if (one_class && list == kListT128) {
         const int64_t segments = one_class == 2 ? P : P / 17;
         return P / kQ8Rows + (segments < E ? segments : E);
@@ -99,7 +100,13 @@ inline int64_t list_capacity(int list, int64_t P, int64_t E, int one_class = 0)
 // A layer on 8-bit activations whose call has more than 32 pairs per expert sends every segment to the tile kernel: most
 // are longer than the streaming kernel's 16 rows, and the streaming launch, a grid of (experts x channel tiles) that
 // finds next to nothing, costs more than the few short tiles (DeepSeek-V3 shape, 8192 tokens: 83 us of 4.3 ms).
-inline int q8_one_class(int64_t P, int64_t E) { return P > 32 * E ? 2 : 1; }
+// A small call on a layer whose weights all fit the caches is bound by its launches: one streaming launch per stage takes
+// every segment (64 tokens, 16 experts of 1024 x 512, top-2: 34.8 us with tile launches of their own, 26 without).
+inline int q8_one_class(int64_t P, int64_t E, int64_t hidden, int64_t inter)
+{
+    if (P <= 512 && E * 3 * hidden * inter <= (64ll << 20)) return 3;
+    return P > 32 * E ? 2 : 1;
+}
 // Item i of the one-class cut of a segment of n rows (n > 16) into `items`: its first row and its rows.
 constexpr int q8_items(int n) { return (n + kQ8Rows - 1) / kQ8Rows; }
 __host__ __device__ inline void q8_item(int n, int items, int i, int *first, int *rows)
@@ -148,6 +155,12 @@ struct PackArgs {
     uint64_t *activation;     // [E] running sum of counts over calls, or nullptr
     int32_t *tile_items_host; // pinned host word that receives the number of tile items cut, or nullptr
     WorkLists lists;
+    // 16-bit rows to quantise beside the routing (see launch_pack), or nullptr
+    const void *quant_x = nullptr;      // [quant_T, quant_H], quant_H a multiple of 64
+    int64_t quant_T = 0;
+    int32_t quant_H = 0, quant_act = 0;
+    uint8_t *quant_q = nullptr;
+    float *quant_scale = nullptr;
 };
 constexpr int kPackChunk = 4096;   // pairs per workgroup
 constexpr int kPackThreads = 256;
@@ -155,7 +168,9 @@ constexpr int kMaxExperts = 1024;
 
 // writes *err itself (one kernel of every pack stores the call's word: nothing to clear first,
 // no memset node: graph-capture safe)
-void launch_pack(const PackArgs &a, hipStream_t s);
+// Returns whether the rows of a.quant_x have been quantised on the way: the one-workgroup form of the step leaves the
+// chip idle, and further workgroups of the same launch take the rows.
+bool launch_pack(const PackArgs &a, hipStream_t s);
 // work lists for one segment [0, n) of expert e (per-expert forward)
 void launch_single_lists(const WorkLists &lists, int32_t expert, int32_t n, bool wide, hipStream_t s);
 // lists that hold the one segment (expert, rows row0 .. row0+n-1) and nothing else; mode 0: the usual

@@ -15,6 +15,7 @@
 // (calls of at most 4096 pairs run all of it in one workgroup, pack_fused)
 // plus a coalesced row gather (assemble_seq_tensors, executor.rs:112-133).
 #include "ek_internal.h"
+#include "ek_quant.h"
 
 namespace ek {
 
@@ -104,6 +105,11 @@ __device__ __forceinline__ SegmentCut cut_segment(int32_t n, int32_t one_class)
 {
     SegmentCut c;
     if (one_class) {
+        if (one_class == 3) {
+            c.n128 = c.n64 = c.n32 = 0;
+            c.ns = (n + kWideRows - 1) / kWideRows;
+            return c;
+        }
         const bool tile = one_class == 2 ? n > 0 : n > 16;
         c.n128 = tile ? q8_items(n) : 0;
         c.n64 = c.n32 = 0;
@@ -117,7 +123,7 @@ __device__ __forceinline__ SegmentCut cut_segment(int32_t n, int32_t one_class)
     c.ns = r > 0 && r <= 16;
     return c;
 }
-__device__ __forceinline__ bool in_one_class(const WorkLists &l, int32_t n) { return l.one_class == 2 ? n > 0 : l.one_class && n > 16; }
+__device__ __forceinline__ bool in_one_class(const WorkLists &l, int32_t n) { return l.one_class == 2 ? n > 0 : l.one_class == 1 && n > 16; }
 __device__ __forceinline__ WorkItem q8_work_item(int32_t e, int32_t seg0, int32_t n, int32_t items, int32_t i)
 {
     int32_t first, rows;
@@ -130,6 +136,11 @@ __device__ __forceinline__ void emit_items(const WorkLists &l, int32_t e, int32_
     if (in_one_class(l, n)) {
         const int32_t items = q8_items(n);
         for (int32_t i = 0; i < items; ++i) l.items[kListT128][p128 + i] = q8_work_item(e, seg0, n, items, i);
+        return;
+    }
+    if (l.one_class == 3) {
+        for (int32_t i = 0; i * kWideRows < n; ++i)
+            l.items[kListStream][ps + i] = WorkItem{e, seg0 + i * kWideRows, min(kWideRows, n - i * kWideRows), 0};
         return;
     }
     const int32_t full = n >> 7, r = n & 127;
@@ -340,9 +351,9 @@ __global__ __launch_bounds__(kPackThreads) void pack_rank_kernel(PackArgs a, int
 // leaving LDS, and no separate clear of the error word.  16 wavefronts; wave w
 // owns the consecutive pairs [w*sub, (w+1)*sub) and keeps them in registers.
 constexpr int kPackFusedMax = 4096;
-__global__ __launch_bounds__(1024) void pack_fused_kernel(PackArgs a, int nbits)
+__device__ __forceinline__ void pack_fused(const PackArgs &a, int nbits, int32_t *lds)
 {
-    extern __shared__ int32_t lds[];          // wbase[16][E], then wave_tot5[16][5], err
+    // lds: wbase[16][E], then wave_tot5[16][5], err
     int32_t (*wave_tot5)[5] = (int32_t (*)[5])(lds + 16 * a.E);
     int32_t *lerr = lds + 16 * a.E + 80;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -423,7 +434,46 @@ __global__ __launch_bounds__(1024) void pack_fused_kernel(PackArgs a, int nbits)
     }
 }
 
-void launch_pack(const PackArgs &a, hipStream_t s)
+__global__ __launch_bounds__(1024) void pack_fused_kernel(PackArgs a, int nbits)
+{
+    extern __shared__ int32_t pack_lds[];
+    pack_fused(a, nbits, pack_lds);
+}
+
+// Workgroup 0 packs, the others quantise 16 rows each, one wave a row.
+template <typename T>
+__global__ __launch_bounds__(1024) void pack_quant_kernel(PackArgs a, int nbits)
+{
+    extern __shared__ int32_t pack_lds[];
+    if (blockIdx.x == 0) {
+        pack_fused(a, nbits, pack_lds);
+        return;
+    }
+    typedef T V8 __attribute__((ext_vector_type(8)));
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)(blockIdx.x - 1) * 16 + (threadIdx.x >> 6);
+    if (row >= a.quant_T) return;
+    const V8 *x = (const V8 *)((const T *)a.quant_x + row * a.quant_H);
+    uint32_t mb = 0;
+    for (int c = lane; c < a.quant_H / 8; c += 64) {
+        const V8 v = x[c];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mb = max(mb, __builtin_bit_cast(uint32_t, (float)v[j]) & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) mb = max(mb, (uint32_t)__shfl_xor((int)mb, d));
+    const QuantRow q(__builtin_bit_cast(float, mb));
+    for (int c = lane; c < a.quant_H / 8; c += 64) {
+        const V8 v = x[c];
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
+        *(uint2 *)(a.quant_q + row * a.quant_H + c * 8) = q.codes(f);
+    }
+    if (lane == 0) a.quant_scale[row] = q.scale();
+}
+
+bool launch_pack(const PackArgs &a, hipStream_t s)
 {
     if (a.P <= 0) {
         // offsets and counts must still be defined (all zero)
@@ -431,7 +481,7 @@ void launch_pack(const PackArgs &a, hipStream_t s)
         z.nblocks = 0;
         z.P = 0;
         hipLaunchKernelGGL(pack_scan_kernel, dim3(1), dim3(1024), 0, s, z);
-        return;
+        return false;
     }
     int nbits = 0;
     while ((1 << nbits) < a.E) ++nbits;
@@ -440,12 +490,19 @@ void launch_pack(const PackArgs &a, hipStream_t s)
     // a single CU's memory pipeline then takes every scattered store of perm and row_token.)
     const size_t lds_bytes = sizeof(int32_t) * (16 * (size_t)a.E + 96);
     if (a.P <= kPackFusedMax && lds_bytes <= 65536) {
+        if (a.quant_x) {
+            const dim3 grid((unsigned)(1 + (a.quant_T + 15) / 16));
+            if (a.quant_act == 0) hipLaunchKernelGGL(pack_quant_kernel<__bf16>, grid, dim3(1024), lds_bytes, s, a, nbits);
+            else hipLaunchKernelGGL(pack_quant_kernel<_Float16>, grid, dim3(1024), lds_bytes, s, a, nbits);
+            return true;
+        }
         hipLaunchKernelGGL(pack_fused_kernel, dim3(1), dim3(1024), lds_bytes, s, a, nbits);
-        return;
+        return false;
     }
     hipLaunchKernelGGL(pack_hist_kernel, dim3(a.nblocks), dim3(kPackThreads), 0, s, a);
     hipLaunchKernelGGL(pack_scan_kernel, dim3(1), dim3(1024), 0, s, a);
     hipLaunchKernelGGL(pack_rank_kernel, dim3(a.nblocks), dim3(kPackThreads), 0, s, a, nbits);
+    return false;
 }
 
 // Xp[j, :] = x[row_token[j], :], 16 bytes per lane, one workgroup per row slice.

@@ -342,7 +342,8 @@ ek_status create_layer(const ek_cfg *cfg, int64_t pmax, ek_layer **out)
         const int64_t min_rows[ek::kNumLists] = {1, 17, 33, 65};
         int64_t cap = rows_max / min_rows[l] + (l == ek::kListStream ? 264 : 1);
         if (l == ek::kListStream && cap > 65535) cap = 65535;
-        if (L->act8 && l == ek::kListT128) cap = rows_max / 17 + 1;     // every segment's remainder joins this list
+        // (8-bit activations: every segment of more than 16 rows, or, from 16 rows per expert on, of any length)
+        if (L->act8 && l == ek::kListT128) cap = rows_max / 14 + 2;
         if (cap < ek::list_capacity(l, rows_max, E + 1, L->act8) + 1) cap = ek::list_capacity(l, rows_max, E + 1, L->act8) + 1;
         L->ws.list_cap[l] = cap;
         A((void **)&L->ws.lists.items[l], sizeof(ek::WorkItem) * cap, "work list");
@@ -697,6 +698,9 @@ ek_status static_scratch_setup(int dev)
     return EK_OK;
 }
 
+// How a layer call of P pairs is cut (the same for pack, an appended shared segment, the launches and the lists' sizes).
+int one_class_of(const ek_layer *L, int64_t P) { return L->act8 ? ek::q8_one_class(P, L->cfg.n_experts, L->cfg.hidden, L->cfg.inter) : 0; }
+
 // Lays a workspace for T tokens of layer L out in `base` (capacity `cap` bytes).  Returns the bytes
 // needed; W is valid only if they fit.
 size_t carve_workspace(const ek_layer *L, int64_t T, unsigned char *base, size_t cap, Workspace *W)
@@ -720,7 +724,7 @@ size_t carve_workspace(const ek_layer *L, int64_t T, unsigned char *base, size_t
     W->wide_items = (ek::WorkItem *)take(sizeof(ek::WorkItem) * kSharedWideItems);
     W->wide_count = (int32_t *)take(sizeof(int32_t) * ek::kNumLists);
     for (int l = 0; l < ek::kNumLists; ++l) {
-        W->list_cap[l] = ek::list_capacity(l, rows, E + 1, L->act8) + (l == ek::kListStream ? 264 : 1);
+        W->list_cap[l] = ek::list_capacity(l, rows, E + 1, one_class_of(L, P)) + (l == ek::kListStream ? 264 : 1);
         W->lists.items[l] = (ek::WorkItem *)take(sizeof(ek::WorkItem) * (size_t)W->list_cap[l]);
     }
     W->lists.one_class = W->slists.one_class = L->act8;
@@ -897,8 +901,7 @@ ek_status copy_route_out(ek_layer *L, const Workspace &W, const ek_route_out *r,
     return EK_OK;
 }
 
-// The work lists of a layer call of P pairs (the same cut for pack, an appended shared segment and the launches).
-int one_class_of(const ek_layer *L, int64_t P) { return L->act8 ? ek::q8_one_class(P, L->cfg.n_experts, L->cfg.hidden, L->cfg.inter) : 0; }
+// The work lists of a layer call of P pairs.
 ek::WorkLists lists_of(const ek_layer *L, const Workspace &W, int64_t P)
 {
     ek::WorkLists l = W.lists;
@@ -1728,7 +1731,8 @@ ek_status ek_layer_expert_forward(ek_layer *layer, int32_t expert, const void *x
             }
             // the ordinary cut's tile items: full 128-row tiles and a remainder of more than 16 rows
             const int64_t wide_items = (n + ek::kWideRows - 1) / ek::kWideRows;
-            const bool wide = ek::wide_cut_pays((n >> 7) + ((n & 127) > 16), n, H, layer->cfg.inter) &&
+            const bool wide = (layer->act8 ? n > 16 && ek::q8_wide_cut_pays(n, ek::q8_items((int)n), n, H, layer->cfg.inter)
+                                           : ek::wide_cut_pays((n >> 7) + ((n & 127) > 16), n, H, layer->cfg.inter)) &&
                               wide_items <= layer->ws.list_cap[ek::kListStream];
             ek::launch_single_lists(layer->ws.lists, expert, (int32_t)n, wide, s);
             if (layer->act8) {
@@ -1805,11 +1809,13 @@ ek_status ek_layer_experts_forward(ek_layer *layer, int32_t n_calls, const int32
             // Work lists cut on the host exactly as the pack kernels cut them: a call is one
             // segment (ek_internal.h, "work lists").
             std::vector<ek::WorkItem> items[ek::kNumLists];
-            int64_t row0 = 0, tile_items = 0, wide_items = 0, short_items = 0;
+            int64_t row0 = 0, tile_items = 0, wide_items = 0, short_items = 0, q8_tiles = 0, q8_rows = 0, longest = 0;
             for (int i = 0; i < n_calls; ++i) {
                 tile_items += (rows[i] >> 7) + ((rows[i] & 127) > 16);
                 wide_items += (rows[i] + ek::kWideRows - 1) / ek::kWideRows;
                 short_items += (rows[i] & 127) > 0 && (rows[i] & 127) <= 16;
+                if (rows[i] > 16) { q8_tiles += ek::q8_items((int)rows[i]); q8_rows += rows[i]; }
+                longest = std::max(longest, rows[i]);
             }
             // The wide cut spares a batch the tile kernel's long, nearly empty launch.  When the batch
             // also has many short requests, their streaming chain (one pass over an expert's weights
@@ -1820,7 +1826,8 @@ ek_status ek_layer_experts_forward(ek_layer *layer, int32_t n_calls, const int32
             const int wb = layer->w8 ? 1 : 2;
             const double cover_us = (double)short_items * 3.0 * (double)H * (double)layer->cfg.inter * wb / 6.5e6;
             const double tiled_us = ek::tile_call_us(H, layer->cfg.inter);
-            const bool wide = ek::wide_cut_pays(tile_items, P, H, layer->cfg.inter) && cover_us < 0.5 * tiled_us &&
+            const bool wide = (layer->act8 ? ek::q8_wide_cut_pays(q8_rows, q8_tiles, longest, H, layer->cfg.inter)
+                                           : ek::wide_cut_pays(tile_items, P, H, layer->cfg.inter)) && cover_us < 0.5 * tiled_us &&
                               wide_items <= layer->ws.list_cap[ek::kListStream];
             for (int i = 0; i < n_calls; ++i) {
                 const int32_t n = (int32_t)rows[i], full = n >> 7, r = n & 127;

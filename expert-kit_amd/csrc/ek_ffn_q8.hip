@@ -43,6 +43,12 @@ constexpr int kQ8Slices = 8;
 
 // One workgroup: RS*16 rows x NG*16 channels (of NMAT matrices); its eight waves take an eighth of the
 // contraction each and meet in LDS.  Operands come straight from memory, D chunks ahead.
+//
+// Up to 16 rows (RS = 1) the call is bound by the weights: one channel tile (of up and gate) per workgroup gives the
+// most loads in flight.  Longer items take RS = 2 rows of fragments x 4 chunks of weights: every fragment of the
+// rows is read by N / 64 workgroups instead of N / 16, which is what the call waits for (MI355X, 64 rows of 7168 x 2048:
+// 16.7 us with one tile and 64 rows, 10.9 with two tiles and 32 rows, 12.6 with four; 512 rows: 56, 35 and 24 us; 64 rows
+// of 2048 x 7168: 11.4, 8.2 and 7.2 us).
 template <typename T, int NMAT, int NG, int RS, int D>
 __global__ __launch_bounds__(64 * kQ8Slices) void q8_stream_kernel(Q8Args a, int list, int item_rows)
 {
@@ -685,9 +691,13 @@ static hipError_t launch_lists(const Q8Args &a, const int64_t max_items[kNumList
 {
     const dim3 block(64 * kQ8Slices);
     if (max_items[kListStream] > 0) {
-        const dim3 grid((unsigned)a.NT, (unsigned)max_items[kListStream]);
-        if (wide) hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 4, 2>), grid, block, 0, s, a, kListStream, 0);
-        else hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 1, 2>), grid, block, 0, s, a, kListStream, 0);
+        const unsigned items = (unsigned)max_items[kListStream];
+        constexpr int NG = 4 / NMAT;
+        if (wide)
+            hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, NG, 2, 2>), dim3((unsigned)((a.NT + NG - 1) / NG), items, kWideRows / 32), block, 0, s,
+                               a, kListStream, 0);
+        else
+            hipLaunchKernelGGL((q8_stream_kernel<T, NMAT, 1, 1, 2>), dim3((unsigned)a.NT, items), block, 0, s, a, kListStream, 0);
     }
     if (max_items[kListT128] > 0) {
         const hipError_t e = launch_tiles<T, NMAT>(a, max_items[kListT128], s);
@@ -707,9 +717,12 @@ template <typename T> static hipError_t launch_dense_t(const Q8Args &a, hipStrea
 {
     const int64_t n = a.dense_rows;
     const dim3 block(64 * kQ8Slices);
-    if (n <= 16) hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 1, 2>), dim3((unsigned)a.NT, 1), block, 0, s, a, 0, 16);
-    else if (n <= 128) hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 4, 2>), dim3((unsigned)a.NT, (unsigned)((n + 63) / 64)), block, 0, s, a, 0, 64);
-    else return launch_tiles<T, 1>(a, (n + kQ8Rows - 1) / kQ8Rows, s);
+    if (n <= 16)
+        hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 1, 2>), dim3((unsigned)a.NT, 1), block, 0, s, a, 0, 16);
+    else if (q8_stream_us(n, a.Kdim, a.NT * 16) < q8_tile_us(n, a.Kdim, a.NT * 16))
+        hipLaunchKernelGGL((q8_stream_kernel<T, 1, 4, 2, 2>), dim3((unsigned)((a.NT + 3) / 4), (unsigned)((n + 31) / 32)), block, 0, s, a, 0, 32);
+    else
+        return launch_tiles<T, 1>(a, (n + kQ8Rows - 1) / kQ8Rows, s);
     return hipGetLastError();
 }
 

@@ -97,15 +97,37 @@ inline int64_t list_capacity(int list, int64_t P, int64_t E, int one_class = 0)
     return by_rows < E ? by_rows : E;
 }
 
-// A layer on 8-bit activations whose call has more than 32 pairs per expert sends every segment to the tile kernel: most
-// are longer than the streaming kernel's 16 rows, and the streaming launch, a grid of (experts x channel tiles) that
-// finds next to nothing, costs more than the few short tiles (DeepSeek-V3 shape, 8192 tokens: 83 us of 4.3 ms).
-// A small call on a layer whose weights all fit the caches is bound by its launches: one streaming launch per stage takes
-// every segment (64 tokens, 16 experts of 1024 x 512, top-2: 34.8 us with tile launches of their own, 26 without).
+// How a layer call of P pairs on 8-bit activations is cut (WorkLists::one_class), measured on MI355X:
+//  * 3, a small call on a layer whose weights fit the caches, which is bound by its launches (16 experts of 1024 x 512, top-2,
+//    64 / 512 tokens: 28.5 / 40 us against 32 / 47 with tile launches beside the streaming ones; with weights beyond the
+//    caches the streaming kernel's short form is better: 128 experts of 2048 x 768, 64 tokens 150 against 137 us);
+//  * 2, from 16 pairs per expert on: most segments are longer than the streaming kernel's 16 rows, and a streaming
+//    launch that finds little costs more than the few short tiles (DeepSeek-V3 shape, 512 / 1024 / 2048 tokens: 1905 / 1996 /
+//    2140 us against 2040 / 2066 / 2200; Qwen3 shape, 256 / 1024 tokens: 152 / 210 against 157 / 225);
+//  * 1 otherwise.
 inline int q8_one_class(int64_t P, int64_t E, int64_t hidden, int64_t inter)
 {
-    if (P <= 512 && E * 3 * hidden * inter <= (64ll << 20)) return 3;
-    return P > 32 * E ? 2 : 1;
+    if (P <= 1024 && E * 3 * hidden * inter <= (64ll << 20)) return 3;
+    return P >= 16 * E ? 2 : 1;
+}
+// Estimates of one int8 product of n rows (n > 16) with N channels of K elements, by the streaming and by the tile kernel:
+// the first does ~0.75 POP/s whatever the size, the second up to 2.3 but takes a round of at least one tile's
+// contraction for every 256 tiles.  Fitted on MI355X: 512 rows x 7168 x 2048 24 / 84 us, 1024 x 7168 x 2048 43 / 84, 1024 x
+// 7168 x 4096 82 / 85, 1024 x 2048 x 7168 47 / 36, 2048 x 7168 x 2048 80 / 85, 256 x 2048 x 7168 18 / 32.
+inline double q8_stream_us(int64_t n, int64_t K, int64_t N) { return 5.0 + 2e-6 * (double)n * (double)K * (double)N / 750.0; }
+inline double q8_tiles_us(int64_t items, int64_t item_rows, int64_t K, int64_t N)
+{
+    const int64_t rounds = (items * ((N + 255) / 256) + 255) / 256;
+    const double blocks = (double)((item_rows < kQ8Rows ? item_rows : kQ8Rows) + 31) / 32.0;
+    return (double)rounds * (14.0 + (double)(K + 127) / 128.0 * (0.45 + 0.1 * blocks));
+}
+inline double q8_tile_us(int64_t n, int64_t K, int64_t N) { return q8_tiles_us((n + kQ8Rows - 1) / kQ8Rows, n, K, N); }
+// Per-expert calls: rows in all, and how many tile items of at most item_rows rows they would be: whether both stages
+// are better streamed.
+inline bool q8_wide_cut_pays(int64_t rows, int64_t items, int64_t item_rows, int64_t hidden, int64_t inter)
+{
+    return items > 0 && q8_stream_us(rows, hidden, 2 * inter) + q8_stream_us(rows, inter, hidden) <
+                            q8_tiles_us(items, item_rows, hidden, 2 * inter) + q8_tiles_us(items, item_rows, inter, hidden);
 }
 // Item i of the one-class cut of a segment of n rows (n > 16) into `items`: its first row and its rows.
 constexpr int q8_items(int n) { return (n + kQ8Rows - 1) / kQ8Rows; }

@@ -130,21 +130,24 @@ __device__ __forceinline__ WorkItem q8_work_item(int32_t e, int32_t seg0, int32_
     q8_item(n, items, i, &first, &rows);
     return WorkItem{e, seg0 + first, rows, 0};
 }
-__device__ __forceinline__ void emit_items(const WorkLists &l, int32_t e, int32_t seg0, int32_t n,
-                                           int32_t p128, int32_t p64, int32_t p32, int32_t ps)
+// The items of a segment of n rows from seg0 on, at their positions in the lists: as many of each class as
+// cut_segment says.  The callers' `threads` threads (this one is number `tid`) share the work.
+__device__ __forceinline__ void emit_items(const WorkLists &l, int32_t e, int32_t seg0, int32_t n, int32_t p128, int32_t p64,
+                                           int32_t p32, int32_t ps, int32_t tid = 0, int32_t threads = 1)
 {
-    if (in_one_class(l, n)) {
-        const int32_t items = q8_items(n);
-        for (int32_t i = 0; i < items; ++i) l.items[kListT128][p128 + i] = q8_work_item(e, seg0, n, items, i);
-        return;
-    }
     if (l.one_class == 3) {
-        for (int32_t i = 0; i * kWideRows < n; ++i)
+        for (int32_t i = tid; i * kWideRows < n; i += threads)
             l.items[kListStream][ps + i] = WorkItem{e, seg0 + i * kWideRows, min(kWideRows, n - i * kWideRows), 0};
         return;
     }
+    if (in_one_class(l, n)) {
+        const int32_t items = q8_items(n);
+        for (int32_t i = tid; i < items; i += threads) l.items[kListT128][p128 + i] = q8_work_item(e, seg0, n, items, i);
+        return;
+    }
     const int32_t full = n >> 7, r = n & 127;
-    for (int32_t t = 0; t < full; ++t) l.items[kListT128][p128 + t] = WorkItem{e, seg0 + t * 128, 128, 0};
+    for (int32_t t = tid; t < full; t += threads) l.items[kListT128][p128 + t] = WorkItem{e, seg0 + t * 128, 128, 0};
+    if (tid != 0) return;
     const WorkItem rem{e, seg0 + full * 128, r, 0};
     if (r > 64) l.items[kListT128][p128 + full] = rem;
     else if (r > 32) l.items[kListT64][p64] = rem;
@@ -221,13 +224,7 @@ __global__ __launch_bounds__(256) void segment_lists_kernel(WorkLists l, int32_t
         return;
     }
     const SegmentCut c = cut_segment(n, l.one_class);
-    const int32_t full = n >> 7;
-    if (in_one_class(l, n)) {
-        for (int32_t t = threadIdx.x; t < c.n128; t += 256) l.items[kListT128][t] = q8_work_item(e, row0, n, c.n128, t);
-    } else {
-        for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][t] = WorkItem{e, row0 + t * 128, 128, 0};
-        if (threadIdx.x == 0 && (n & 127)) emit_items(l, e, row0 + full * 128, n & 127, full, 0, 0, 0);    // the remainder, into its class
-    }
+    emit_items(l, e, row0, n, 0, 0, 0, 0, threadIdx.x, 256);
     if (threadIdx.x == 0) {
         l.count[kListT128] = c.n128;
         l.count[kListT64] = c.n64;
@@ -256,14 +253,8 @@ __global__ __launch_bounds__(256) void append_segment_kernel(WorkLists l, int32_
         return;
     }
     const SegmentCut c = cut_segment(n, l.one_class);
-    const int32_t full = n >> 7, r = n & 127;
     for (int32_t t = threadIdx.x; t < n; t += 256) row_token[row0 + t] = t;
-    if (in_one_class(l, n)) {
-        for (int32_t t = threadIdx.x; t < c.n128; t += 256) l.items[kListT128][p128 + t] = q8_work_item(e, row0, n, c.n128, t);
-    } else {
-        for (int32_t t = threadIdx.x; t < full; t += 256) l.items[kListT128][p128 + t] = WorkItem{e, row0 + t * 128, 128, 0};
-        if (threadIdx.x == 0 && r > 0) emit_items(l, e, row0 + full * 128, r, p128 + full, p64, p32, ps);
-    }
+    emit_items(l, e, row0, n, p128, p64, p32, ps, threadIdx.x, 256);
     if (threadIdx.x == 0) {
         l.count[kListT128] = p128 + c.n128;
         l.count[kListT64] = p64 + c.n64;

@@ -597,11 +597,10 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
                 }
                 T4 o;
                 if constexpr (NMAT == 2) {
+                    float gate[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int i = q * 4 + r;
-                        o[r] = swiglu_rounded<T>(v[r], as_fp32((float)acc[rb][1][i] * (xs * ws[1][i])));
-                    }
+                    for (int r = 0; r < 4; ++r) gate[r] = as_fp32((float)acc[rb][1][q * 4 + r] * (xs * ws[1][q * 4 + r]));
+                    o = swiglu4_rounded<T>(v, gate);
                 } else {
                     if (a.bias) {
 #pragma unroll

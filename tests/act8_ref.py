@@ -85,8 +85,10 @@ def product(q, scale, w, w_scale):
 
 
 def quantise(x16):
-    q, s = codes(x16)
-    return q, (x16.float().abs().amax(1) / 127.0)
+    """A row with an infinity or a NaN has codes of 0 and the scale NaN."""
+    finite = x16.float().isfinite().all(1)
+    q, _ = codes(torch.where(finite[:, None], x16, torch.zeros_like(x16)))
+    return q, torch.where(finite, x16.float().abs().amax(1) / 127.0, torch.full_like(finite, float("nan"), dtype=torch.float32))
 
 
 def expert(q, scale, ew, dt):

@@ -255,3 +255,41 @@ def test_errors(ek, cuda):
     assert status(lambda: layer.forward(x, with_1, w)) == C.EK_EXPERT_NOT_FOUND
     assert status(lambda: layer.forward_q8(q, s, with_1, w)) == C.EK_EXPERT_NOT_FOUND
     assert layer.forward_q8(q[:0], s[:0], ids[:0], w[:0]).shape == (0, H)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_every_gate_value(ek, cuda, dt):
+    """Every finite value of the type as the gate's pre-activation, through the tile kernel (all at once) and the
+    streaming one (a few hundred at a time): the row's scale is the value's magnitude, the code of the first column its
+    sign, and an expert for each sign and exponent holds up's scale, so that the product is a normal number."""
+    v = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dt)
+    v = v[v.isfinite()]
+    bits = v.view(torch.int16).int() & 0xffff
+    frac = 7 if dt == torch.bfloat16 else 10
+    eid = (bits >> frac).to(torch.int32)                              # sign and exponent field
+    E, H, I = int(eid.max()) + 1, 128, 64
+    mag = v.abs().float()
+    experts = []
+    layer = ek.HipLayer(H, I, E, 1, act_dtype=dt, w_dtype=torch.int8, max_tokens=len(v), act8=True)
+    lead = {e: float(mag[eid == e].max()) for e in torch.unique(eid).tolist()}
+    unit = lambda rows, cols, at: torch.zeros(rows, cols, dtype=torch.int8).index_put_((torch.tensor(0), torch.tensor(at)), torch.tensor(1, dtype=torch.int8))
+    for e in range(E):
+        m = lead.get(e, 1.0)
+        positive = e < E // 2 and m >= 1.0
+        us = 2.0 ** max(-100.0, min(120.0, (0.0 if positive else 8.0) - float(torch.tensor(m).log2().floor())))
+        w = ek.ExpertWeight(up_w=unit(I, H, 1), gate_w=unit(I, H, 0), down_w=unit(H, I, 0), up_scale=torch.full((I,), us),
+                            gate_scale=torch.ones(I), down_scale=torch.ones(H))
+        experts.append(w)
+        layer.set_expert(e, w)
+    q = torch.zeros(len(v), H, dtype=torch.int8)
+    q[:, 0] = torch.where(v < 0, -1, 1).to(torch.int8)
+    q[:, 1] = 1
+    ids, gw = eid[:, None].contiguous(), torch.ones(len(v), 1)
+    want = ref.layer(q, mag, ids, gw, experts, dt)
+    assert int((want[:, 0] != 0).sum()) > len(v) // 3
+    args = [t.to(cuda) for t in (q, mag, ids, gw)]
+    same(layer.forward_q8(*args), want, "all")
+    for lo in range(0, len(v), 8192):
+        part = slice(lo, lo + 300)
+        same(layer.forward_q8(*[t[part].contiguous() for t in args]), want[part], "a few")
+    layer.close()

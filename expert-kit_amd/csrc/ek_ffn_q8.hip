@@ -718,7 +718,7 @@ template <typename T> static hipError_t launch_dense_t(const Q8Args &a, hipStrea
     const dim3 block(64 * kQ8Slices);
     if (n <= 16)
         hipLaunchKernelGGL((q8_stream_kernel<T, 1, 1, 1, 2>), dim3((unsigned)a.NT, 1), block, 0, s, a, 0, 16);
-    else if (q8_stream_us(n, a.Kdim, a.NT * 16) < q8_tile_us(n, a.Kdim, a.NT * 16))
+    else if (n <= 65535 * 32 && q8_stream_us(n, a.Kdim, a.NT * 16) < q8_tile_us(n, a.Kdim, a.NT * 16))      // (grid.y)
         hipLaunchKernelGGL((q8_stream_kernel<T, 1, 4, 2, 2>), dim3((unsigned)((a.NT + 3) / 4), (unsigned)((n + 31) / 32)), block, 0, s, a, 0, 32);
     else
         return launch_tiles<T, 1>(a, (n + kQ8Rows - 1) / kQ8Rows, s);

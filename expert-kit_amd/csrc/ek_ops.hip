@@ -60,7 +60,7 @@ ek_status load_bytes(void *dst, const void *src, size_t bytes, int32_t mem)
 }
 
 // Rows of one call: one workgroup of up to 1024 threads per row, and a launch holds less than 2^32 threads along a
-// dimension; 64-row groups of the products are numbered by a grid dimension of at most 65535.
+// dimension.
 constexpr int64_t kMaxRows = 65535 * 64;
 
 }  // namespace

@@ -237,6 +237,8 @@ class HipLayer:
             raise C.EKError(C.EK_INVALID_INPUT, "q must be [T, hidden] int8, scale [T] fp32, ids and w [T, top_k] (int32, gate weights), on one device")
         if out is not None and (tuple(out.shape) != tuple(q.shape) or out.dtype != self.act_dtype or out.device != q.device or not out.is_contiguous()):
             raise C.EKError(C.EK_INVALID_INPUT, "out must be a contiguous [T, hidden] tensor of the activation dtype beside q")
+        if q.is_cuda and q.device.index != self.cfg.device_id:
+            raise C.EKError(C.EK_INVALID_INPUT, f"tensors are on {q.device}, the layer on device {self.cfg.device_id}")
         with (_alloc_on(stream) if out is None or return_route or not (q.is_contiguous() and scale.is_contiguous()
                                                                       and ids.is_contiguous() and w.is_contiguous()) else _NO_CTX):
             q, scale, ids, w = q.contiguous(), scale.contiguous(), ids.contiguous(), w.contiguous()

@@ -230,8 +230,9 @@ ek_status ek_layer_forward(ek_layer *layer, const void *x, const int32_t *ids, c
                            int32_t mem, void *stream);
 
 /* ek_layer_forward on rows that are 8-bit already (ek_norm_forward's q and scale): x [T, hidden] int8,
- * x_scale [T] fp32.  The layer was created with EK_CFG_ACT8; everything else as in ek_layer_forward, and
- * the same bits as its call on 16-bit rows whose quantisation is (x, x_scale). */
+ * x_scale [T] fp32; on the device x is 16-byte and x_scale 4-byte aligned.  The layer was created with
+ * EK_CFG_ACT8; everything else as in ek_layer_forward, and the same bits as its call on 16-bit rows whose
+ * quantisation is (x, x_scale). */
 ek_status ek_layer_forward_q8(ek_layer *layer, const void *x, const float *x_scale, const int32_t *ids, const void *w,
                               int32_t w_dtype, int64_t T, void *y, const ek_route_out *route, int32_t mem, void *stream);
 
@@ -509,7 +510,8 @@ ek_status ek_expert_destroy(ek_expert *expert);
  *   y   = rnd16(v)                      for the router's gate product and other 16-bit readers
  *   q, scale = v quantised as above     (from v itself, not from y)
  * rnd16 is the rounding to act_dtype; nothing else is rounded to 16 bits.  q is exactly the definition's
- * (the scale cancels rstd out of it), whatever the order of the sum over the row. */
+ * (the scale cancels rstd out of it), whatever the order of the sum over the row.  The products sum * gain
+ * are taken in fp32: one beyond its range counts as an infinity, one below 2^-126 loses bits. */
 typedef struct ek_norm ek_norm;
 typedef struct ek_norm_cfg {
     int64_t hidden;      /* row length: a positive multiple of 8 */

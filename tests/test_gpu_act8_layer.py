@@ -293,3 +293,45 @@ def test_every_gate_value(ek, cuda, dt):
         part = slice(lo, lo + 300)
         same(layer.forward_q8(*[t[part].contiguous() for t in args]), want[part], "a few")
     layer.close()
+
+
+def test_two_graphs(ek, cuda):
+    """Two captured calls of one layer, of different sizes and so of different cuts, replayed in turn on one stream."""
+    H, I, E, K, dt = 256, 192, 8, 2, torch.bfloat16
+    layer, ws, _ = build(ek, H, I, E, K, dt, 700, seed=70)
+    sizes = (700, 40, 1)
+    data = [[t.to(cuda) for t in call(T, H, E, K, dt, seed=T)] for T in sizes]
+    ys = [layer.forward(*d) for d in data]
+    st, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for d, y in zip(data, ys):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            layer.forward(*d, stream=st, out=y)
+        graphs.append(g)
+    for rep in range(1, 4):
+        fresh = [call(T, H, E, K, dt, seed=T + rep, skew=0.5 * rep) for T in sizes]
+        for d, f in zip(data, fresh):
+            for t, v in zip(d, f):
+                t.copy_(v)
+        for y in ys:
+            y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            for g in graphs:
+                g.replay()
+        torch.cuda.synchronize()
+        for (x, ids, w), y in zip(fresh, ys):
+            same(y, ref.layer(*ref.quantise(x), ids, w, ws, dt), f"replay {rep}, {len(x)} tokens")
+
+
+def test_tensors_of_another_device_are_refused(ek, cuda):
+    from ek_hip import _capi as C
+    H, I, E, K, T, dt = 128, 64, 2, 1, 4, torch.bfloat16
+    layer, _, _ = build(ek, H, I, E, K, dt, T, seed=80)
+    x, ids, w = call(T, H, E, K, dt)
+    q, s = ref.quantise(x)
+    layer.cfg.device_id = 1                                        # (what the object holds; the handle is untouched)
+    with pytest.raises(ek.EKError) as ei:
+        layer.forward_q8(q.to(torch.int8).to(cuda), s.to(cuda), ids.to(cuda), w.to(cuda))
+    assert ei.value.status == C.EK_INVALID_INPUT

@@ -168,3 +168,48 @@ def test_linear_refusals(ek, cuda):
     assert lib.ek_linear_forward(h, p + 1, ds.data_ptr(), 1, p, C.EK_DEVICE, None) == C.EK_INVALID_INPUT
     assert lib.ek_linear_forward(h, None, ds.data_ptr(), 1, p, C.EK_DEVICE, None) == C.EK_INVALID_INPUT
     assert lib.ek_linear_forward(h, None, None, 0, None, C.EK_DEVICE, None) == C.EK_OK
+
+
+@pytest.mark.parametrize("K", [128, 100])
+def test_linear_more_rows_than_one_grid_dimension_counts(ek, cuda, K):
+    """More 32-row groups than 65535: the same rows as in calls of a few (narrow matrices are where such calls are
+    estimated to be faster in 32-row groups)."""
+    n, N = 65535 * 32 + 77, 16
+    _, _, w, ws, _ = make(1, K, N, torch.bfloat16, False, seed=8)
+    op = ek.HipLinear(w.to(cuda), ws.to(cuda), max_rows=n)
+    q = torch.randint(-127, 128, (n, K), device=cuda, dtype=torch.int8)
+    s = torch.rand(n, device=cuda)
+    y = op.forward(q, s)
+    for lo in (0, 65535 * 16 + 3, n - 300):
+        part = slice(lo, lo + 300)
+        check(y[part], q[part].cpu(), s[part].cpu(), w, ws, None, torch.bfloat16)
+    small = ek.HipLinear(w.to(cuda), ws.to(cuda), max_rows=1 << 18)
+    for lo in range(0, n, 1 << 18):
+        part = slice(lo, min(lo + (1 << 18), n))
+        assert torch.equal(y[part], small.forward(q[part].contiguous(), s[part].contiguous()))
+
+
+def test_linear_two_graphs(ek, cuda):
+    """Two captured calls that share the workspace, replayed in turn on one stream with an eager call between."""
+    _, _, w, ws, _ = make(1, 200, 80, torch.float16, False, seed=9)
+    op = ek.HipLinear(w.to(cuda), ws.to(cuda), act_dtype=torch.float16, max_rows=400)
+    xs = [torch.randn(n, 200, device=cuda).half() for n in (400, 19)]
+    ys = [op.forward(x) for x in xs]
+    st, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for x, y in zip(xs, ys):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            op.forward(x, stream=st, out=y)
+        graphs.append(g)
+    for _ in range(3):
+        for x in xs:
+            x.normal_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            for g in graphs * 2:
+                g.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(xs, ys):
+            got = y.clone()
+            assert torch.equal(op.forward(x), got)

@@ -276,7 +276,6 @@ struct RowQuantArgs {
     int32_t q_stride;         // a multiple of 8, at least H
     float eps;
     double inv_h;             // 1 / H
-    bool wide;                // norm: sum the squares in fp64 throughout (an eps below what fp32 squares resolve)
     bool vec;                 // rows of x start on 16-byte boundaries (H a multiple of 8)
 };
 hipError_t launch_row_quant(const RowQuantArgs &a, int act, bool norm, hipStream_t s);

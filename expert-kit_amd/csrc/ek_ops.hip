@@ -237,7 +237,6 @@ ek_status ek_norm_forward(ek_norm *norm, const void *x, const void *residual, in
         ek::RowQuantArgs a{};
         a.gain = norm->gain;
         a.n = n; a.H = (int32_t)H; a.q_stride = (int32_t)H; a.eps = norm->cfg.eps; a.inv_h = 1.0 / (double)H; a.vec = true;
-        a.wide = norm->cfg.eps < 0x1p-80f;
         DeviceGuard dg(norm->cfg.device_id);
         if (!dg.ok) return fail(EK_HIP_ERROR, "hipSetDevice(%d) failed", norm->cfg.device_id);
         if (mem == EK_DEVICE) {

@@ -10,7 +10,8 @@
 // and quant8 (ek_quant.h) gives it exactly, ties included.
 //
 // Bound: HBM.  A row is read once into registers by one workgroup, which reduces its sum
-// of squares and its maximum together and writes everything from registers.
+// of squares and its maximum together and writes everything from registers: 8192 rows of 7168 with residual and all
+// outputs, 529 MB, 96 us on MI355X = 5.5 TB/s (a copy of 4 GiB reaches 4.7).
 #include "ek_internal.h"
 #include "ek_mfma.h"
 #include "ek_quant.h"
@@ -30,7 +31,7 @@ enum RowMode {
 template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
 
 // 8 columns as they come from memory.  All loads of a row are issued before anything is computed (a branch between them
-// makes each wait for the one before: 183 us instead of 106 for 8192 rows of 7168); groups past the row's end
+// makes each wait for the one before: 183 us against 106 for 8192 rows of 7168); groups past the row's end
 // re-read its last one and count as zeros.
 template <typename T, int MODE> struct RawCols {
     typename Vec8<T>::type x, residual, gain;
@@ -68,6 +69,37 @@ template <typename T, int MODE> struct RawCols {
     }
 };
 
+// p * rstd (rstd = hi + lo) as fp32 values whose rounding to T is that of the product itself.  The fp32 product is the
+// nearest, so its rounding to T is right but where it lies on a tie of T that the product does not lie on, or where
+// the result is below T's normal numbers (other ties).  There the fp64 product goes to the one of its two fp32 neighbours
+// that is odd (and so on no tie).  One group of 8 in 8192 (bf16) or 1024 (fp16) takes that way.
+template <typename T>
+__device__ __forceinline__ void round_to_odd_ties(const float *p, float hi, float lo, double rstd, float *t)
+{
+    constexpr bool BF = std::is_same<T, __bf16>::value;
+    constexpr uint32_t kLow = BF ? 1u << 16 : 1u << 13;              // fp32 steps between neighbours of T
+    constexpr uint32_t kNormal = BF ? 0x00800000u : 0x38800000u;     // T's least normal number
+    uint32_t tie = kLow, least = ~0u;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        t[j] = __builtin_fmaf(p[j], hi, p[j] * lo);
+        const uint32_t b = __builtin_bit_cast(uint32_t, t[j]);
+        tie = min(tie, (b - kLow / 2) & (kLow - 1));
+        least = min(least, 2 * b - 1);                               // (zero is exact)
+    }
+    if (__builtin_expect(tie == 0 || least < 2 * kNormal - 1, 0)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const double d = (double)p[j] * rstd;
+            const float f = (float)d;
+            uint32_t b = __builtin_bit_cast(uint32_t, f);
+            if ((b & 1) == 0 && (double)f != d && __builtin_fabs(d) < 0x1p128)
+                b += __builtin_fabs(d) > __builtin_fabs((double)f) ? 1u : ~0u;
+            t[j] = __builtin_bit_cast(float, b);
+        }
+    }
+}
+
 // WPR waves per row, RPB rows per workgroup.  NV > 0: a thread keeps its NV groups of 8 columns in registers; NV = 0:
 // rows too long for that are read twice (the second time mostly from L2).
 template <typename T, int MODE, int NV, int WPR, int RPB>
@@ -84,49 +116,17 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
     for (int64_t row = RPB > 1 ? (int64_t)blockIdx.x * RPB + wave : blockIdx.x; row < a.n; row += (int64_t)gridDim.x * RPB) {
         float p[KEEP][8];
         V8 r[KEEP];
-        // Squares are summed in fp32 over 8 columns and in fp64 from there; a row whose squares do not fit fp32 (values
-        // beyond 2^63 in a bf16 row) is summed again in fp64 from the first, so that no finite row overflows.
+        // Squares are summed in fp64: no finite row overflows, and rstd is good for y's rounding (below).
         double ss = 0.0;
         uint32_t mb = 0;                                   // max |p| as bits: NaN orders behind infinity
-        auto take = [&](const float *pv, const V8 &rv, bool wide) {
-            float q = 0.f;
+        auto take = [&](const float *pv, const V8 &rv) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if constexpr (NORM) {
-                    const float f = (float)rv[j];
-                    if (wide) ss = __builtin_fma((double)f, (double)f, ss);
-                    else q = __builtin_fmaf(f, f, q);
+                    const double f = (double)(float)rv[j];
+                    ss = __builtin_fma(f, f, ss);
                 }
                 mb = max(mb, __builtin_bit_cast(uint32_t, pv[j]) & 0x7fffffffu);
-            }
-            if constexpr (NORM) ss += (double)q;
-        };
-        auto take_row = [&](bool wide) {
-            if constexpr (NV > 0) {
-#pragma unroll
-                for (int u = 0; u < NV; ++u) take(p[u], r[u], wide);
-            } else {
-                for (int c = tid; c < nvec; c += THREADS) {
-                    RawCols<T, MODE> raw;
-                    raw.load(a, row, c, nvec);
-                    r[0] = raw.values(c, a.H, p[0]);
-                    take(p[0], r[0], wide);
-                }
-            }
-#pragma unroll
-            for (int d = 32; d >= 1; d >>= 1) {
-                if constexpr (NORM) ss += __shfl_xor(ss, d);
-                mb = max(mb, (uint32_t)__shfl_xor((int)mb, d));
-            }
-            if constexpr (WPR > 1) {
-                __shared__ double s_ss[WPR];
-                __shared__ uint32_t s_m[WPR];
-                if (lane == 0) { s_ss[wave] = ss; s_m[wave] = mb; }
-                __syncthreads();
-                ss = s_ss[0]; mb = s_m[0];
-#pragma unroll
-                for (int w = 1; w < WPR; ++w) { ss += s_ss[w]; mb = max(mb, s_m[w]); }
-                __syncthreads();                           // (the same LDS serves the next sums)
             }
         };
         if constexpr (NV > 0) {
@@ -134,23 +134,42 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
 #pragma unroll
             for (int u = 0; u < NV; ++u) raw[u].load(a, row, u * THREADS + tid, nvec);
 #pragma unroll
-            for (int u = 0; u < NV; ++u) r[u] = raw[u].values(u * THREADS + tid, a.H, p[u]);
-        }
-        take_row(NORM && a.wide);
-        if constexpr (NORM) {
-            if (!a.wide && !(ss < __builtin_huge_val())) {  // (the same for every thread of the row)
-                ss = 0.0;
-                take_row(true);
+            for (int u = 0; u < NV; ++u) {
+                r[u] = raw[u].values(u * THREADS + tid, a.H, p[u]);
+                take(p[u], r[u]);
             }
+        } else {
+            for (int c = tid; c < nvec; c += THREADS) {
+                RawCols<T, MODE> raw;
+                raw.load(a, row, c, nvec);
+                r[0] = raw.values(c, a.H, p[0]);
+                take(p[0], r[0]);
+            }
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) {
+            if constexpr (NORM) ss += __shfl_xor(ss, d);
+            mb = max(mb, (uint32_t)__shfl_xor((int)mb, d));
+        }
+        if constexpr (WPR > 1) {
+            __shared__ double s_ss[WPR];
+            __shared__ uint32_t s_m[WPR];
+            if (lane == 0) { s_ss[wave] = ss; s_m[wave] = mb; }
+            __syncthreads();
+            ss = s_ss[0]; mb = s_m[0];
+#pragma unroll
+            for (int w = 1; w < WPR; ++w) { ss += s_ss[w]; mb = max(mb, s_m[w]); }
+            __syncthreads();                           // (the same LDS serves the next sums)
         }
         const float m = __builtin_bit_cast(float, mb);
         float rstd = 1.f, rlow = 0.f;
+        double y1 = 1.0;
         if constexpr (NORM) {
-            // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40), as two fp32
+            // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40), and as two fp32
             // values, so that a product with it rounds once
             const double ms = ss * a.inv_h + (double)a.eps;
             const double y0 = __builtin_amdgcn_rsq(ms);
-            const double y1 = y0 * (1.5 - 0.5 * ms * y0 * y0);    // NaN for a row with an infinity or NaN
+            y1 = y0 * (1.5 - 0.5 * ms * y0 * y0);                 // NaN for a row with an infinity or NaN
             rstd = (float)y1;
             rlow = (float)(y1 - (double)rstd);
         }
@@ -162,9 +181,11 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
                 const int64_t at = row * (a.H >> 3) + c;
                 if (a.sum) ((V8 *)a.sum)[at] = rv;
                 if (a.y) {
+                    float t[8];
+                    round_to_odd_ties<T>(pv, rstd, rlow, y1, t);
                     V8 o;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = (T)as_fp32(__builtin_fmaf(pv[j], rstd, pv[j] * rlow));
+                    for (int j = 0; j < 8; ++j) o[j] = (T)as_fp32(t[j]);
                     ((V8 *)a.y)[at] = o;
                 }
             }

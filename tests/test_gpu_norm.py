@@ -176,3 +176,19 @@ def test_norm_refusals(ek, cuda):
     assert lib.ek_norm_forward(h, None, None, 1, None, p, None, None, C.EK_DEVICE, None) == C.EK_INVALID_INPUT
     assert lib.ek_norm_forward(h, p, None, 1, None, p, None, None, C.EK_HOST, torch.cuda.Stream().cuda_stream) == C.EK_INVALID_INPUT
     assert lib.ek_norm_forward(h, p, None, 0, None, p, None, None, C.EK_DEVICE, None) == C.EK_OK                     # no rows
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,H,scale", [(400, 2048, 1.0), (60, 7168, 1.0), (9, 33000, 1.0), (500, 512, 2e-7)])
+def test_norm_rounds_y_once(ek, cuda, dt, n, H, scale):
+    """y is the definition's value rounded to 16 bits once: equal wherever that value is further from a tie than the
+    kernel's 64-bit arithmetic is inexact (2^-40, and the reference's own 2^-50); scale: rows so small that y is subnormal in fp16."""
+    x, r, gain = make(n, H, dt, seed=12)
+    gain = (gain.float() * scale).to(dt)
+    out = ek.HipNorm(gain).forward(x.to(cuda), r.to(cuda))
+    _, v, _, _ = ref.norm(x, r, gain, EPS)
+    low, high = ref.rounded(v * (1 - 2.0 ** -38), dt), ref.rounded(v * (1 + 2.0 ** -38), dt)
+    y = out.y.cpu()
+    clear = low == high
+    assert int((~clear).sum()) <= 8
+    assert torch.equal(y[clear], low[clear])

@@ -27,42 +27,23 @@ __global__ __launch_bounds__(kPackThreads) void pack_hist_kernel(PackArgs a)
     const int64_t base = (int64_t)blockIdx.x * kPackChunk;
     const int64_t end = min(base + (int64_t)kPackChunk, a.P);
     // (ids out of range are left out; the scan kernel sees that the counts do not add up to P)
-    for (int64_t p = base + threadIdx.x; p < end; p += kPackThreads) {
-        const int32_t id = a.ids[p];
-        if ((uint32_t)id < (uint32_t)a.E) atomicAdd(&hist[id], 1);
+    int32_t id[kPackChunk / kPackThreads];                // all loads in flight at once
+#pragma unroll
+    for (int u = 0; u < kPackChunk / kPackThreads; ++u) {
+        const int64_t p = base + u * kPackThreads + threadIdx.x;
+        id[u] = p < end ? a.ids[p] : -1;
     }
+#pragma unroll
+    for (int u = 0; u < kPackChunk / kPackThreads; ++u)
+        if ((uint32_t)id[u] < (uint32_t)a.E) atomicAdd(&hist[id[u]], 1);
     __syncthreads();
     for (int i = threadIdx.x; i < a.E; i += kPackThreads)
         a.block_hist[(int64_t)blockIdx.x * a.E + i] = hist[i];
 }
 
-// Exclusive prefix sum of one int per thread over a 1024-thread workgroup:
-// shuffles inside each wavefront, then the 16 wave totals through LDS.
-// Returns the exclusive prefix; *total receives the workgroup sum.
-__device__ __forceinline__ int32_t block_exclusive_scan(int32_t v, int32_t *wave_tot, int32_t *total)
-{
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int32_t incl = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int32_t up = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += up;
-    }
-    __syncthreads();   // wave_tot may still be read from a previous scan
-    if (lane == 63) wave_tot[wave] = incl;
-    __syncthreads();
-    int32_t base = 0, sum = 0;
-    for (int w = 0; w < 16; ++w) {
-        const int32_t t = wave_tot[w];
-        if (w < wave) base += t;
-        sum += t;
-    }
-    *total = sum;
-    return base + incl - v;
-}
-
-// The same for five ints per thread at once (one pair of barriers instead of five): the offsets
-// and the four work lists' positions of the one-workgroup pack.  wave_tot: [16][5].
+// Exclusive prefix sums of five ints per thread over a 1024-thread workgroup (the offsets and the four
+// work lists' positions), with one pair of barriers: shuffles inside each wavefront, then the 16 wave
+// totals through LDS.  wave_tot: [16][5].
 __device__ __forceinline__ void block_exclusive_scan5(const int32_t (&v)[5], int32_t (*wave_tot)[5],
                                                       int32_t (&excl)[5], int32_t (&total)[5])
 {
@@ -92,6 +73,7 @@ __device__ __forceinline__ void block_exclusive_scan5(const int32_t (&v)[5], int
             if (w < wave) base += t;
             sum += t;
         }
+        asm volatile("" : "+v"(base), "+v"(sum));  // sums of this place: the sixteen totals need not live until their use
         total[i] = sum;
         excl[i] = base + incl[i] - v[i];
     }
@@ -158,9 +140,10 @@ __device__ __forceinline__ void emit_items(const WorkLists &l, int32_t e, int32_
 // One workgroup of 1024 threads; thread e owns expert e.
 __global__ __launch_bounds__(1024) void pack_scan_kernel(PackArgs a)
 {
-    __shared__ int32_t wave_tot[16];
+    __shared__ int32_t wave_tot[16][5];
     const int e = threadIdx.x;
     int32_t total = 0;
+    const bool absent = e < a.E && a.slabs != nullptr && a.slabs[e].upgate == nullptr;
     if (e < a.E) {
         // exclusive prefix over chunks, 16 chunks' counts in flight at a time (one dependent load
         // per chunk made this kernel's time: 10 us at 9 chunks)
@@ -178,10 +161,12 @@ __global__ __launch_bounds__(1024) void pack_scan_kernel(PackArgs a)
         a.counts[e] = total;
         if (a.activation) a.activation[e] += (uint64_t)total;
     }
-    const bool unloaded = e < a.E && total > 0 && a.slabs != nullptr && a.slabs[e].upgate == nullptr;
-    const int any_unloaded = __syncthreads_or(unloaded);
-    int32_t sum;
-    const int32_t off = block_exclusive_scan(total, wave_tot, &sum);
+    const int any_unloaded = __syncthreads_or(absent && total > 0);
+    const SegmentCut c = cut_segment(total, a.lists.one_class);
+    const int32_t v5[5] = {total, c.n128, c.n64, c.n32, c.ns};
+    int32_t ex[5], tot5[5];
+    block_exclusive_scan5(v5, wave_tot, ex, tot5);
+    const int32_t off = ex[0], sum = tot5[0];
     if (e < a.E) a.offsets[e] = off;
     if (e == 0) {
         a.offsets[a.E] = sum;
@@ -189,19 +174,13 @@ __global__ __launch_bounds__(1024) void pack_scan_kernel(PackArgs a)
         a.err[0] = ((int64_t)sum != a.P ? 1 : 0) | (any_unloaded ? 2 : 0);
     }
     if (a.lists.count == nullptr) return;
-    const SegmentCut c = cut_segment(total, a.lists.one_class);
-    int32_t s128, s64, s32, ss;
-    const int32_t p128 = block_exclusive_scan(c.n128, wave_tot, &s128);
-    const int32_t p64 = block_exclusive_scan(c.n64, wave_tot, &s64);
-    const int32_t p32 = block_exclusive_scan(c.n32, wave_tot, &s32);
-    const int32_t ps = block_exclusive_scan(c.ns, wave_tot, &ss);
-    if (e < a.E && total > 0) emit_items(a.lists, e, off, total, p128, p64, p32, ps);
+    if (e < a.E && total > 0) emit_items(a.lists, e, off, total, ex[1], ex[2], ex[3], ex[4]);
     if (e == 0) {
-        a.lists.count[kListT128] = s128;
-        a.lists.count[kListT64] = s64;
-        a.lists.count[kListT32] = s32;
-        a.lists.count[kListStream] = ss;
-        if (a.tile_items_host) *a.tile_items_host = s128 + s64 + s32;
+        a.lists.count[kListT128] = tot5[1];
+        a.lists.count[kListT64] = tot5[2];
+        a.lists.count[kListT32] = tot5[3];
+        a.lists.count[kListStream] = tot5[4];
+        if (a.tile_items_host) *a.tile_items_host = tot5[1] + tot5[2] + tot5[3];
     }
 }
 
@@ -281,28 +260,35 @@ void launch_segment_lists(const WorkLists &lists, int32_t expert, int32_t row0, 
     hipLaunchKernelGGL(segment_lists_kernel, dim3(1), dim3(256), 0, s, lists, expert, row0, n, row_token, mode);
 }
 
-__global__ __launch_bounds__(kPackThreads) void pack_rank_kernel(PackArgs a, int nbits)
+// 16 waves per chunk of 4096 pairs: a wave's 256 pairs are four dependent steps on its counters (65536 pairs on MI355X:
+// 10 us, 20 with four waves that load the ids again at every step).
+constexpr int kRankThreads = 1024;
+__global__ __launch_bounds__(kRankThreads) void pack_rank_kernel(PackArgs a, int nbits)
 {
-    constexpr int kWaves = kPackThreads / 64;
+    constexpr int kWaves = kRankThreads / 64;
     constexpr int kSub = kPackChunk / kWaves;   // pairs per wave, consecutive
-    __shared__ int32_t wbase[kWaves][kMaxExperts];
+    extern __shared__ int32_t rank_lds[];                 // wbase[kWaves][E]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < kWaves * kMaxExperts; i += kPackThreads) (&wbase[0][0])[i] = 0;
-    __syncthreads();
+    int32_t *wbase = rank_lds + wave * a.E;
     const int64_t start = (int64_t)blockIdx.x * kPackChunk + (int64_t)wave * kSub;
+    // the wave's ids, loaded once: one memory latency instead of one per 64 pairs in either loop below
+    int32_t ids[kSub / 64];
+#pragma unroll
     for (int it = 0; it < kSub / 64; ++it) {
         const int64_t p = start + it * 64 + lane;
-        if (p < a.P) {
-            const int32_t id = a.ids[p];
-            if ((uint32_t)id < (uint32_t)a.E) atomicAdd(&wbase[wave][id], 1);
-        }
+        ids[it] = p < a.P ? a.ids[p] : -1;
     }
+    for (int i = threadIdx.x; i < kWaves * a.E; i += kRankThreads) rank_lds[i] = 0;
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += kPackThreads) {
+#pragma unroll
+    for (int it = 0; it < kSub / 64; ++it)
+        if ((uint32_t)ids[it] < (uint32_t)a.E) atomicAdd(&wbase[ids[it]], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += kRankThreads) {
         int32_t run = a.offsets[e] + a.block_hist[(int64_t)blockIdx.x * a.E + e];
         for (int w = 0; w < kWaves; ++w) {
-            const int32_t t = wbase[w][e];
-            wbase[w][e] = run;
+            const int32_t t = rank_lds[w * a.E + e];
+            rank_lds[w * a.E + e] = run;
             run += t;
         }
     }
@@ -310,15 +296,12 @@ __global__ __launch_bounds__(kPackThreads) void pack_rank_kernel(PackArgs a, int
     // Each wave walks its own consecutive pairs 64 at a time; lanes holding
     // the same expert id find each other with one ballot per id bit, so the
     // rank inside the group is the number of lower lanes in the group.
+#pragma unroll
     for (int it = 0; it < kSub / 64; ++it) {
         const int64_t p = start + it * 64 + lane;
-        int32_t id = 0;
-        bool valid = false;
-        if (p < a.P) {
-            id = a.ids[p];
-            valid = (uint32_t)id < (uint32_t)a.E;
-            if (!valid) a.inv_perm[p] = -1;
-        }
+        const int32_t id = ids[it];
+        const bool valid = (uint32_t)id < (uint32_t)a.E;
+        if (!valid && p < a.P) a.inv_perm[p] = -1;
         uint64_t m = __ballot(valid);
         for (int b = 0; b < nbits; ++b) {
             const bool bit = (id >> b) & 1;
@@ -327,12 +310,12 @@ __global__ __launch_bounds__(kPackThreads) void pack_rank_kernel(PackArgs a, int
         }
         if (valid) {
             const int32_t rank = __popcll(m & ((1ull << lane) - 1ull));
-            const int32_t pos = wbase[wave][id] + rank;
+            const int32_t pos = wbase[id] + rank;
             const bool leader = (m >> lane) == 1ull;   // highest lane of the group
-            if (leader) wbase[wave][id] = pos + 1;
+            if (leader) wbase[id] = pos + 1;
             a.perm[pos] = (int32_t)p;
             a.inv_perm[p] = pos;
-            a.row_token[pos] = (int32_t)(p / a.K);
+            a.row_token[pos] = (int32_t)((uint32_t)p / (uint32_t)a.K);
         }
     }
 }
@@ -420,7 +403,7 @@ __device__ __forceinline__ void pack_fused(const PackArgs &a, int nbits, int32_t
             if (leader) lds[wave * a.E + id[it]] = pos + 1;
             a.perm[pos] = (int32_t)p;
             a.inv_perm[p] = pos;
-            a.row_token[pos] = (int32_t)(p / a.K);
+            a.row_token[pos] = (int32_t)((uint32_t)p / (uint32_t)a.K);
         }
     }
 }
@@ -492,7 +475,7 @@ bool launch_pack(const PackArgs &a, hipStream_t s)
     }
     hipLaunchKernelGGL(pack_hist_kernel, dim3(a.nblocks), dim3(kPackThreads), 0, s, a);
     hipLaunchKernelGGL(pack_scan_kernel, dim3(1), dim3(1024), 0, s, a);
-    hipLaunchKernelGGL(pack_rank_kernel, dim3(a.nblocks), dim3(kPackThreads), 0, s, a, nbits);
+    hipLaunchKernelGGL(pack_rank_kernel, dim3(a.nblocks), dim3(kRankThreads), sizeof(int32_t) * (kRankThreads / 64) * (size_t)a.E, s, a, nbits);
     return false;
 }
 

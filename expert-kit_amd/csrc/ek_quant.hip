@@ -69,37 +69,6 @@ template <typename T, int MODE> struct RawCols {
     }
 };
 
-// p * rstd (rstd = hi + lo) as fp32 values whose rounding to T is that of the product itself.  The fp32 product is the
-// nearest, so its rounding to T is right but where it lies on a tie of T that the product does not lie on, or where
-// the result is below T's normal numbers (other ties).  There the fp64 product goes to the one of its two fp32 neighbours
-// that is odd (and so on no tie).  One group of 8 in 8192 (bf16) or 1024 (fp16) takes that way.
-template <typename T>
-__device__ __forceinline__ void round_to_odd_ties(const float *p, float hi, float lo, double rstd, float *t)
-{
-    constexpr bool BF = std::is_same<T, __bf16>::value;
-    constexpr uint32_t kLow = BF ? 1u << 16 : 1u << 13;              // fp32 steps between neighbours of T
-    constexpr uint32_t kNormal = BF ? 0x00800000u : 0x38800000u;     // T's least normal number
-    uint32_t tie = kLow, least = ~0u;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        t[j] = __builtin_fmaf(p[j], hi, p[j] * lo);
-        const uint32_t b = __builtin_bit_cast(uint32_t, t[j]);
-        tie = min(tie, (b - kLow / 2) & (kLow - 1));
-        least = min(least, 2 * b - 1);                               // (zero is exact)
-    }
-    if (__builtin_expect(tie == 0 || least < 2 * kNormal - 1, 0)) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const double d = (double)p[j] * rstd;
-            const float f = (float)d;
-            uint32_t b = __builtin_bit_cast(uint32_t, f);
-            if ((b & 1) == 0 && (double)f != d && __builtin_fabs(d) < 0x1p128)
-                b += __builtin_fabs(d) > __builtin_fabs((double)f) ? 1u : ~0u;
-            t[j] = __builtin_bit_cast(float, b);
-        }
-    }
-}
-
 // WPR waves per row, RPB rows per workgroup.  NV > 0: a thread keeps its NV groups of 8 columns in registers; NV = 0:
 // rows too long for that are read twice (the second time mostly from L2).
 template <typename T, int MODE, int NV, int WPR, int RPB>
@@ -116,7 +85,7 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
     for (int64_t row = RPB > 1 ? (int64_t)blockIdx.x * RPB + wave : blockIdx.x; row < a.n; row += (int64_t)gridDim.x * RPB) {
         float p[KEEP][8];
         V8 r[KEEP];
-        // Squares are summed in fp64: no finite row overflows, and rstd is good for y's rounding (below).
+        // Squares are summed in fp64: no finite row overflows, and y is the definition's value as the nearest fp32 number, rounded to 16 bits.
         double ss = 0.0;
         uint32_t mb = 0;                                   // max |p| as bits: NaN orders behind infinity
         auto take = [&](const float *pv, const V8 &rv) {
@@ -163,13 +132,12 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
         }
         const float m = __builtin_bit_cast(float, mb);
         float rstd = 1.f, rlow = 0.f;
-        double y1 = 1.0;
         if constexpr (NORM) {
-            // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40), and as two fp32
+            // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40), as two fp32
             // values, so that a product with it rounds once
             const double ms = ss * a.inv_h + (double)a.eps;
             const double y0 = __builtin_amdgcn_rsq(ms);
-            y1 = y0 * (1.5 - 0.5 * ms * y0 * y0);                 // NaN for a row with an infinity or NaN
+            const double y1 = y0 * (1.5 - 0.5 * ms * y0 * y0);    // NaN for a row with an infinity or NaN
             rstd = (float)y1;
             rlow = (float)(y1 - (double)rstd);
         }
@@ -181,11 +149,9 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
                 const int64_t at = row * (a.H >> 3) + c;
                 if (a.sum) ((V8 *)a.sum)[at] = rv;
                 if (a.y) {
-                    float t[8];
-                    round_to_odd_ties<T>(pv, rstd, rlow, y1, t);
                     V8 o;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = (T)as_fp32(t[j]);
+                    for (int j = 0; j < 8; ++j) o[j] = (T)as_fp32(__builtin_fmaf(pv[j], rstd, pv[j] * rlow));
                     ((V8 *)a.y)[at] = o;
                 }
             }

@@ -507,7 +507,7 @@ ek_status ek_expert_destroy(ek_expert *expert);
 /* RMS norm of the residual stream, in front of an MoE block (and of attention):
  *   sum = rnd16(x + residual)           (x itself when residual is NULL)
  *   v   = sum * gain / sqrt(mean(sum^2) + eps)
- *   y   = rnd16(v)                      for the router's gate product and other 16-bit readers
+ *   y   = rnd16(v)                      for the router's gate product and other 16-bit readers (by way of fp32)
  *   q, scale = v quantised as above     (from v itself, not from y)
  * rnd16 is the rounding to act_dtype; nothing else is rounded to 16 bits.  q is exactly the definition's
  * (the scale cancels rstd out of it), whatever the order of the sum over the row.  The products sum * gain

@@ -112,13 +112,3 @@ def layer(q, scale, ids, w, experts, dt, shared=None):
         acc = acc + (p if w.dtype == torch.float32 else p.to(dt).float())
     y = acc.to(dt)
     return y if shared is None else (y.float() + expert(q, scale, shared, dt).float()).to(dt)
-
-
-def rounded(v, dt):
-    """64-bit values rounded to a 16-bit type once, ties to even (a conversion by way of fp32 rounds twice)."""
-    f = v.float()
-    b = f.view(torch.int32)
-    inexact = (f.double() != v) & f.isfinite() & v.isfinite()
-    step = torch.where(v.abs() > f.double().abs(), 1, -1).to(torch.int32)
-    b = torch.where(inexact & (b % 2 == 0), b + step, b)                   # the odd one of the two fp32 neighbours
-    return b.view(torch.float32).to(dt)

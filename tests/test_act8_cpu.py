@@ -75,19 +75,3 @@ def test_linear_create_refusals(ek):
     assert lib.ek_linear_forward(None, None, None, 0, None, 0, None) == C.EK_INVALID_INPUT
     assert lib.ek_linear_shape(None, None, None) == C.EK_INVALID_INPUT
     assert lib.ek_linear_destroy(None) == C.EK_INVALID_INPUT
-
-
-@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
-def test_rounding_once(dt):
-    """ref.rounded against the nearest of the two neighbours, found by distance, next to ties and among subnormal numbers."""
-    g = torch.Generator().manual_seed(1)
-    base = torch.cat([torch.randn(500, generator=g), torch.randn(500, generator=g) * 1e-6]).to(dt)
-    up = torch.nextafter(base, torch.full_like(base, float("inf")))
-    mid = (base.double() + up.double()) / 2
-    for rel in (0.0, 2.0 ** -30, -2.0 ** -30, 2.0 ** -45):
-        v = mid * (1 + rel)
-        got = ref.rounded(v, dt).double()
-        dl, du = (v - base.double()).abs(), (v - up.double()).abs()
-        even = (base.view(torch.int16) & 1) == 0
-        want = torch.where((dl < du) | ((dl == du) & even), base.double(), up.double())
-        assert torch.equal(got, want)

@@ -180,14 +180,14 @@ def test_norm_refusals(ek, cuda):
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n,H,scale", [(400, 2048, 1.0), (60, 7168, 1.0), (9, 33000, 1.0), (500, 512, 2e-7)])
-def test_norm_rounds_y_once(ek, cuda, dt, n, H, scale):
-    """y is the definition's value rounded to 16 bits once: equal wherever that value is further from a tie than the
-    kernel's 64-bit arithmetic is inexact (2^-40, and the reference's own 2^-50); scale: rows so small that y is subnormal in fp16."""
+def test_norm_y_is_the_nearest_fp32_value_rounded(ek, cuda, dt, n, H, scale):
+    """y by way of fp32: equal wherever the definition's value is further from a border of fp32 than the kernel's arithmetic
+    is inexact (2^-40 for rstd, and the product's low part, 2^-48); scale: rows so small that y is subnormal in fp16."""
     x, r, gain = make(n, H, dt, seed=12)
     gain = (gain.float() * scale).to(dt)
     out = ek.HipNorm(gain).forward(x.to(cuda), r.to(cuda))
     _, v, _, _ = ref.norm(x, r, gain, EPS)
-    low, high = ref.rounded(v * (1 - 2.0 ** -38), dt), ref.rounded(v * (1 + 2.0 ** -38), dt)
+    low, high = (v * (1 - 2.0 ** -38)).float().to(dt), (v * (1 + 2.0 ** -38)).float().to(dt)
     y = out.y.cpu()
     clear = low == high
     assert int((~clear).sum()) <= 8

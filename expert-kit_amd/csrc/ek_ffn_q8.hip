@@ -395,6 +395,10 @@ __device__ __forceinline__ void dma16(const void *gaddr, uint32_t lds_addr)     
 {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(gaddr), "s"(lds_addr) : "memory");
 }
+__device__ __forceinline__ void dma4(const void *gaddr, uint32_t lds_addr)      // lane l's 4 bytes at lds_addr + 4 l
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(gaddr), "s"(lds_addr) : "memory");
+}
 template <int N> __device__ __forceinline__ void wait_vmcnt() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 // The wave has its LDS reads back before it lets the others overwrite what it read.
 __device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
@@ -409,14 +413,32 @@ static_assert(kQ8Rows == 64 * kQ8Waves && 4 * 64 == 64 * kQ8Waves, "one row and 
 
 __device__ __forceinline__ int q8_key(int row) { return (row & 7) ^ ((row >> 3) & 1); }
 
+// (what names the tile is the same for every lane: scalar loads)
+typedef const __attribute__((address_space(4))) int32_t *ConstInts;
+typedef const __attribute__((address_space(4))) uint64_t *ConstWords;
+
+// slab_at: the expert's ExpertSlab.  It and the rows' numbers are asked for together.
 template <typename T, int NMAT, int RB>
-__device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab, int row0, int n, int cblock, uint8_t *lds)
+__device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int row0, int n, int cblock, uint8_t *lds)
 {
-    const uint8_t *wmat = NMAT == 2 ? slab.upgate : slab.down;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, kh = lane >> 5, j = lane & 15;
     const int KT = a.Kdim >> 6, nfull = KT >> 1, ns = (KT + 1) >> 1;
+    // the rows' numbers in x: of thread tid's scale, and of the DMAs (instruction q brings rows 8q .. 8q+7, lane l piece
+    // (l & 7) ^ key of row 8q + l / 8); rows past the item re-read its last one
+    int32_t row_sc = row0 + min(tid, n - 1), row[RB];
+#pragma unroll
+    for (int i = 0; i < RB; ++i) row[i] = row0 + min((wave * RB + i) * 8 + (lane >> 3), n - 1);
+    if (a.rows) {
+        row_sc = a.rows[row_sc];
+#pragma unroll
+        for (int i = 0; i < RB; ++i) row[i] = a.rows[row[i]];
+    }
+    const ExpertSlab slab{(const uint8_t *)slab_at[0], (const uint8_t *)slab_at[1], (const float *)slab_at[2], (const float *)slab_at[3],
+                          (const float *)slab_at[4]};
+    const uint8_t *wmat = NMAT == 2 ? slab.upgate : slab.down;
+    if (wmat == nullptr) return;                                 // expert not loaded: the call has been flagged
     const uint32_t lds_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
     constexpr int kStep = 2 * NMAT * kChunkBytes;            // bytes from one step's weights to the next's
     // the wave's first 16-channel tile; block cb: matrix cb of tiles nt0, nt0 + 1, or tiles nt0 + 2 cb, + 1
@@ -426,29 +448,6 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
     for (int cb = 0; cb < 2; ++cb) {
         const int nt = min(nt0 + (NMAT == 2 ? 0 : cb * 2) + (l32 >> 4), a.NT - 1);   // tiles past the last recompute it
         wp[cb] = wmat + ((int64_t)nt * KT * NMAT + (NMAT == 2 ? cb : 0)) * kChunkBytes + (kh * 16 + j) * 16;
-    }
-    // rows: DMA instruction q brings rows 8q .. 8q+7, lane l piece (l & 7) ^ key of row 8q + l / 8
-    const uint8_t *xsrc[RB];
-    int32_t tail_fix[RB];            // half a step at the end: lanes of its upper half re-read the lower one
-#pragma unroll
-    for (int i = 0; i < RB; ++i) {
-        const int r = (wave * RB + i) * 8 + (lane >> 3);
-        const int rr = min(r, n - 1);                            // rows past the item re-read its last one
-        const int64_t row = a.rows ? (int64_t)a.rows[row0 + rr] : (int64_t)(row0 + rr);
-        const int piece = (lane & 7) ^ q8_key(r);
-        xsrc[i] = a.x + row * a.Kdim + piece * 16;
-        tail_fix[i] = (piece & 4) ? 64 : 0;
-    }
-    // scales of the tile's rows and of its matrix channels, for the epilogue: one of each per thread, by way of LDS
-    float *scales = (float *)(lds + kQ8Scales);
-    float sc_row, sc_ch, sc_bias = 0.f;
-    {
-        const int rr = min(tid, n - 1);
-        sc_row = a.x_scale[a.rows ? (int64_t)a.rows[row0 + rr] : (int64_t)(row0 + rr)];
-        const int ch0 = cblock * kQ8Waves * (NMAT == 2 ? 32 : 64);          // up: threads 0 .. 127, gate: 128 .. 255
-        const int ch = min(ch0 + (NMAT == 2 ? tid & 127 : tid), a.NT * 16 - 1);
-        sc_ch = (NMAT == 2 ? (tid < 128 ? slab.s_up : slab.s_gate) : slab.s_down)[ch];
-        if (NMAT == 1 && a.bias) sc_bias = a.bias[ch];
     }
     const int bkey = q8_key(l32);
     int boff[4];
@@ -463,13 +462,6 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[rb][cb][r] = 0;
 
-    // DMAs of step s into its stage (steps past the last one repeat it: in bounds, into a stage that is free)
-    auto issue = [&](int s, int stage) {
-        const int sc = min(s, ns - 1);
-#pragma unroll
-        for (int i = 0; i < RB; ++i)
-            dma16(xsrc[i] + (int64_t)sc * 128 - (sc == nfull ? tail_fix[i] : 0), lds_base + stage * kQ8Stage + (wave * RB + i) * 1024);
-    };
     constexpr int D = kQ8Stages;
     uint4 w[D][4][2];
     // one k-group's weights of the step wp points to; hi: from there to the step's second chunk
@@ -501,20 +493,49 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, const ExpertSlab &slab,
                 acc[rb][cb] = __builtin_amdgcn_mfma_i32_32x32x32_i8(q, b[kg & 1][rb], acc[rb][cb], 0, 0, 0);
         }
     };
-#pragma unroll
-    for (int t = 0; t < D; ++t) {
-        issue(t, t);
+    // The first step's weights, then the scales and the rows, whose numbers have come meanwhile, then the other steps' weights.
+    auto first_w = [&](int t) {
         const int hi = t == 0 ? NMAT * kChunkBytes : move_w(t);              // (K >= 128: the first step is whole)
 #pragma unroll
         for (int kg = 0; kg < 4; ++kg) {
             load_w(t, kg, hi);
             __builtin_amdgcn_sched_barrier(0);       // in the order in which they are used
         }
+    };
+    first_w(0);
+    // the scales of the tile's rows and of its matrix channels, for the epilogue: one of each per thread
+    float *scales = (float *)(lds + kQ8Scales);
+    {
+        const int ch0 = cblock * kQ8Waves * (NMAT == 2 ? 32 : 64);          // up: threads 0 .. 127, gate: 128 .. 255
+        const int ch = min(ch0 + (NMAT == 2 ? tid & 127 : tid), a.NT * 16 - 1);
+        const uint32_t at = lds_base + kQ8Scales + wave * 256;
+        dma4(a.x_scale + row_sc, at);
+        dma4((NMAT == 2 ? (tid < 128 ? slab.s_up : slab.s_gate) : slab.s_down) + ch, at + 1024);
+        if (NMAT == 1) {
+            if (a.bias) dma4(a.bias + ch, at + 2048);
+            else scales[512 + tid] = 0.f;
+        }
     }
-    scales[tid] = sc_row;
-    scales[256 + tid] = sc_ch;
-    if (NMAT == 1) scales[512 + tid] = sc_bias;
-    wait_vmcnt<(D - 1) * RB + 8 * D>();   // step 0's DMAs have landed: everything else is younger
+    const uint8_t *xsrc[RB];
+    int32_t tail_fix[RB];            // half a step at the end: lanes of its upper half re-read the lower one
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+        const int piece = (lane & 7) ^ q8_key((wave * RB + i) * 8 + (lane >> 3));
+        xsrc[i] = a.x + (int64_t)row[i] * a.Kdim + piece * 16;
+        tail_fix[i] = (piece & 4) ? 64 : 0;
+    }
+    // DMAs of step s into its stage (steps past the last one repeat it: in bounds, into a stage that is free)
+    auto issue = [&](int s, int stage) {
+        const int sc = min(s, ns - 1);
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+            dma16(xsrc[i] + (int64_t)sc * 128 - (sc == nfull ? tail_fix[i] : 0), lds_base + stage * kQ8Stage + (wave * RB + i) * 1024);
+    };
+#pragma unroll
+    for (int t = 0; t < D; ++t) issue(t, t);
+#pragma unroll
+    for (int t = 1; t < D; ++t) first_w(t);
+    wait_vmcnt<(D - 1) * (RB + 8)>();  // step 0's DMAs have landed: the other steps' are younger, and their weights
     block_barrier();
     read_b(0, 0);
 
@@ -643,10 +664,7 @@ template <typename T, int NMAT>
 __global__ __launch_bounds__(64 * kQ8Waves, 1) void q8_tile_kernel(Q8Args a, int cblocks, int group)
 {
     extern __shared__ __align__(1024) uint8_t q8_lds[];
-    // (what names the tile is the same for every lane: scalar loads)
-    typedef const __attribute__((address_space(4))) int32_t *cint;
-    typedef const __attribute__((address_space(4))) uint64_t *cptr;
-    const uint32_t items = a.dense_rows > 0 ? (uint32_t)((a.dense_rows + kQ8Rows - 1) / kQ8Rows) : (uint32_t)((cint)(uintptr_t)a.lists.count)[kListT128];
+    const uint32_t items = a.dense_rows > 0 ? (uint32_t)((a.dense_rows + kQ8Rows - 1) / kQ8Rows) : (uint32_t)((ConstInts)(uintptr_t)a.lists.count)[kListT128];
     const uint32_t tiles = items * (uint32_t)cblocks, per = (tiles + 7) >> 3, at = blockIdx.x >> 3;
     const uint32_t tile = (blockIdx.x & 7) * per + at;
     if (at >= per || tile >= tiles) return;
@@ -658,12 +676,10 @@ __global__ __launch_bounds__(64 * kQ8Waves, 1) void q8_tile_kernel(Q8Args a, int
         row0 = it * kQ8Rows;
         n = (int)min((int64_t)kQ8Rows, a.dense_rows - row0);
     } else {
-        const cint item = (cint)(uintptr_t)(a.lists.items[kListT128] + it);
+        const ConstInts item = (ConstInts)(uintptr_t)(a.lists.items[kListT128] + it);
         e = item[0]; row0 = item[1]; n = item[2];
     }
-    const cptr sp = (cptr)(uintptr_t)(a.slabs + e);
-    const ExpertSlab slab{(const uint8_t *)sp[0], (const uint8_t *)sp[1], (const float *)sp[2], (const float *)sp[3], (const float *)sp[4]};
-    if ((NMAT == 2 ? slab.upgate : slab.down) == nullptr) return;          // expert not loaded: the call has been flagged
+    const ConstWords slab = (ConstWords)(uintptr_t)(a.slabs + e);
     switch ((n + 31) >> 5) {
     case 1: q8_tile<T, NMAT, 1>(a, slab, row0, n, cblock, q8_lds); break;
     case 2: q8_tile<T, NMAT, 2>(a, slab, row0, n, cblock, q8_lds); break;

@@ -542,41 +542,44 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int
     // Step s (slot = stage = s % 3), one k-group after the other: the rows' fragments of the next k-group are read, the
     // products of this one run, its weight registers are loaded for step s + 3.  Before the last k-group, whose
     // fragments have been read, the workgroup meets: every wave is done with this stage, which takes step s + 3,
-    // and step s + 1 is in LDS, whose first fragments are read behind the last k-group's products.  A step's DMAs are
-    // followed by at least RB + 16 younger loads when they are waited for: every step issues the same number of loads,
-    // those for steps past the last repeat what is there.  The fences keep the compiler from gathering the loads at the
-    // end of the step, and from converting all weights at its start (which would wait for the last of them).
-    auto step = [&](int s, auto slot_c) {
+    // and step s + 1 is in LDS, whose first fragments are read behind the last k-group's products.  In a full round a step's
+    // DMAs are followed by at least RB + 16 younger loads when they are waited for: every step issues the same number of
+    // loads, those for steps past the last repeat what is there (the loop carries them, so the compiler cannot drop them).
+    // The one or two steps behind the last full round (REST) load nothing and wait for everything.  The fences keep the
+    // compiler from gathering the loads at the end of the step, and from converting all weights at its start (which
+    // would wait for the last of them).
+    auto step = [&](int s, auto slot_c, auto rest_c) {
         constexpr int SLOT = decltype(slot_c)::value, NEXT = (SLOT + 1) % D;
-        const int hi = move_w(s + D);
+        constexpr bool REST = decltype(rest_c)::value;
+        const int hi = REST ? 0 : move_w(s + D);
 #pragma unroll
         for (int kg = 0; kg < 4; ++kg) {
             if (kg == 3) {
-                wait_vmcnt<(D - 2) * (RB + 8) + 8>();
+                wait_vmcnt<REST ? 0 : (D - 2) * (RB + 8) + 8>();
                 block_barrier();
-                issue(s + D, SLOT);
+                if constexpr (!REST) issue(s + D, SLOT);
                 read_b(NEXT, 0);
             } else {
                 read_b(SLOT, kg + 1);
             }
             if (kg < 2 || s < nfull) products(SLOT, kg);             // half a step at the end has two k-groups
-            load_w(SLOT, kg, hi);
+            if constexpr (!REST) load_w(SLOT, kg, hi);
             __builtin_amdgcn_sched_group_barrier(0x100, RB, 0);      // the LDS reads first
             __builtin_amdgcn_sched_group_barrier(0x008, 2 * RB, 0);
-            __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);
+            if constexpr (!REST) __builtin_amdgcn_sched_group_barrier(0x020, 2, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     // D steps a round (the loop has no other way out, so that the compiler's own waits are those of a full ring)
     auto steps = [&](auto self, int s, auto slot_c) -> void {
         constexpr int SLOT = decltype(slot_c)::value;
-        step(s, slot_c);
+        step(s, slot_c, std::false_type{});
         if constexpr (SLOT + 1 < D) self(self, s + 1, std::integral_constant<int, SLOT + 1>{});
     };
     auto rest = [&](auto self, int s, auto slot_c) -> void {
         constexpr int SLOT = decltype(slot_c)::value;
         if (s >= ns) return;
-        step(s, slot_c);
+        step(s, slot_c, std::true_type{});
         if constexpr (SLOT + 2 < D) self(self, s + 1, std::integral_constant<int, SLOT + 1>{});
     };
     int s = 0;

@@ -1,5 +1,8 @@
 """Layers on 8-bit activations (EK_CFG_ACT8) against the kernels' arithmetic restated on the CPU: the integer
 sums are exact and every other operation is an IEEE fp32 one, so the outputs are compared bit for bit."""
+import os
+import random
+
 import pytest
 import torch
 
@@ -335,3 +338,27 @@ def test_tensors_of_another_device_are_refused(ek, cuda):
     with pytest.raises(ek.EKError) as ei:
         layer.forward_q8(q.to(torch.int8).to(cuda), s.to(cuda), ids.to(cuda), w.to(cuda))
     assert ei.value.status == C.EK_INVALID_INPUT
+
+
+@pytest.mark.parametrize("draw", range(24))
+def test_drawn_layers(ek, cuda, draw):
+    """Sizes, routings, types and shared experts drawn from a seed (EKSEED=n draws others)."""
+    rng = random.Random(int(os.environ.get("EKSEED", "0")) * 1000 + draw)
+    H = rng.choice([8 * rng.randint(1, 80), 64 * rng.randint(2, 24)])
+    I = rng.choice([rng.randint(1, 300), 64 * rng.randint(2, 16)])
+    E = rng.choice([1, 2, 3, 7, 16, 40])
+    K, T = rng.randint(1, min(E, 8)), rng.choice([1, rng.randint(2, 70), rng.randint(60, 700), rng.randint(500, 1500)])
+    dt, w32 = rng.choice([torch.bfloat16, torch.float16]), rng.random() < 0.5
+    whole = H % 64 == 0 and H >= 128 and I % 64 == 0 and I >= 128        # (padded layers take a shared expert of their own width only)
+    shared_inter = rng.choice([None, None, I, 64 * rng.randint(2, 6) if whole else I])
+    layer, ws, shared = build(ek, H, I, E, K, dt, T, seed=draw, shared_inter=shared_inter)
+    x, ids, w = call(T, H, E, K, dt, seed=draw, skew=rng.choice([0.0, 0.7, 2.0]), w32=w32)
+    q, s = ref.quantise(x)
+    want = ref.layer(q, s, ids, w, ws, dt, shared)
+    what = f"H={H} I={I} E={E} K={K} T={T} {dt} shared={shared_inter}"
+    dx, dids, dw, dq, ds = [t.to(cuda) for t in (x, ids, w, q.to(torch.int8), s)]
+    same(layer.forward(dx, dids, dw), want, what)
+    y, _ = layer.forward_q8(dq, ds, dids, dw, return_route=True)
+    same(y, want, what + " (8-bit rows, tables)")
+    e, n = rng.randrange(E), rng.randint(1, T)
+    same(layer.expert_forward(e, dx[:n]), ref.expert(q[:n], s[:n], ws[e], dt), what + f" (expert {e}, {n} rows)")

@@ -517,19 +517,20 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int
         }
     }
     const uint8_t *xsrc[RB];
-    int32_t tail_fix[RB];            // half a step at the end: lanes of its upper half re-read the lower one
+    // half a step at the end: lanes of its upper half re-read the lower one (q8_key of a row differs from lane >> 3 in its
+    // lowest bit alone, so a lane has pieces of the same half in every row)
+    const int32_t tail_fix = (((lane & 7) ^ (lane >> 3)) & 4) ? 64 : 0;
 #pragma unroll
     for (int i = 0; i < RB; ++i) {
         const int piece = (lane & 7) ^ q8_key((wave * RB + i) * 8 + (lane >> 3));
         xsrc[i] = a.x + (int64_t)row[i] * a.Kdim + piece * 16;
-        tail_fix[i] = (piece & 4) ? 64 : 0;
     }
     // DMAs of step s into its stage (steps past the last one repeat it: in bounds, into a stage that is free)
     auto issue = [&](int s, int stage) {
         const int sc = min(s, ns - 1);
 #pragma unroll
         for (int i = 0; i < RB; ++i)
-            dma16(xsrc[i] + (int64_t)sc * 128 - (sc == nfull ? tail_fix[i] : 0), lds_base + stage * kQ8Stage + (wave * RB + i) * 1024);
+            dma16(xsrc[i] + (int64_t)sc * 128 - (sc == nfull ? tail_fix : 0), lds_base + stage * kQ8Stage + (wave * RB + i) * 1024);
     };
 #pragma unroll
     for (int t = 0; t < D; ++t) issue(t, t);
@@ -595,6 +596,8 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int
     const int nch = min(a.N - c0, NC);
     constexpr int PPR = NC / 8;                                  // 16-byte pieces per row
     const bool whole = nch == NC && (a.out_stride & 7) == 0;
+    // (the lane's number asked for again: kept through the steps it was the one register too many)
+    const int elane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     typedef T T4 __attribute__((ext_vector_type(4)));
     float ws[2][16], bias[2][16];
 #pragma unroll
@@ -643,7 +646,7 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
         for (int i = 0; i < 32 * PPR / 64; ++i) {
-            const int r = (i * 64 + lane) / PPR, c = (lane % PPR) * 8;
+            const int r = (i * 64 + elane) / PPR, c = (elane % PPR) * 8;
             if (rb * 32 + r >= n) continue;
             T *orow = (T *)a.out + (int64_t)(row0 + rb * 32 + r) * a.out_stride + c0;
             const uint8_t *src = scratch + r * kQ8ScratchPitch + c * 2;

@@ -926,7 +926,7 @@ ek::PackArgs pack_args(ek_layer *L, const Workspace &W, const int32_t *ids, int6
     a.row_token = W.row_token;
     a.err = W.err;
     a.activation = check_loaded ? L->d_activation : nullptr;
-    a.tile_items_host = check_loaded ? L->d_tile_items : nullptr;
+    a.tile_items_host = check_loaded && !L->act8 ? L->d_tile_items : nullptr;      // (read by the 16-bit path alone)
     if (check_loaded) a.lists = lists_of(L, W, P);
     else a.lists = ek::WorkLists{{nullptr, nullptr, nullptr, nullptr}, nullptr};
     return a;
@@ -1287,7 +1287,7 @@ ek_status enqueue_forward(ek_layer *L, const Workspace &W, const void *x, const 
         ek::PairArgs pa{};
         pa.ids = ids; pa.P = (int32_t)P; pa.K = K; pa.n_experts = E; pa.shared = shared_cut(L, T).shared ? 1 : 0;
         pa.x16 = x_scale ? nullptr : x; pa.h = W.h; pa.w = w; pa.w_f32 = w_f32; pa.y = y;
-        pa.err = W.err; pa.activation = L->d_activation; pa.tile_items_host = L->d_tile_items;
+        pa.err = W.err; pa.activation = L->d_activation;
         for (int i = 1; i <= 2 && ev; ++i) EK_HIP(hipEventRecord(ev[i], s));     // (both kernels count as the down phase)
         EK_HIP(ek::launch_pairs_q8(up, down, pa, L->act, s));
         if (ev) EK_HIP(hipEventRecord(ev[3], s));

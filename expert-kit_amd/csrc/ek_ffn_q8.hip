@@ -198,10 +198,7 @@ __device__ __forceinline__ void pair_bookkeeping(const PairArgs &pa, const Exper
     const bool unloaded = ok && slabs[id].upgate == nullptr;
     const uint64_t any_bad = __ballot(bad), any_unloaded = __ballot(unloaded);
     if (ok && pa.activation) atomicAdd((unsigned long long *)&pa.activation[id], 1ull);
-    if (lane == 0) {
-        pa.err[0] = (any_bad ? 1 : 0) | (any_unloaded ? 2 : 0);
-        if (pa.tile_items_host) *pa.tile_items_host = 0;
-    }
+    if (lane == 0) pa.err[0] = (any_bad ? 1 : 0) | (any_unloaded ? 2 : 0);
 }
 
 // The codes of one row of n 16-bit values (n a multiple of 64) by the THREADS lanes that hold it, into LDS; returns the

@@ -314,7 +314,6 @@ struct PairArgs {
     void *y;                  // [T, N]
     int32_t *err;             // the call's bookkeeping, as the pack kernel would store it
     uint64_t *activation;
-    int32_t *tile_items_host;
 };
 // LDS holds a token's rows of h as codes (and stage 1's row of x)
 inline bool q8_pairs_fit(int64_t P, int64_t K, int64_t hidden, int64_t inter)

@@ -230,7 +230,7 @@ void free_layer(ek_layer *L)
     delete L;
 }
 
-constexpr int64_t kAct8MaxK = 131072;     // longest contraction of an int8 product
+constexpr int64_t kAct8MaxK = 131072;     // longest contraction of an int8 product: 128 * 128 * 131072 = 2^31 (ek_ffn_q8.hip)
 
 ek_status validate_cfg(const ek_cfg *c)
 {
@@ -242,7 +242,6 @@ ek_status validate_cfg(const ek_cfg *c)
     if (c->flags & ~(EK_CFG_BLOCK_SCALES | EK_CFG_ACT8)) return fail(EK_INVALID_INPUT, "unknown flags 0x%x", c->flags);
     if ((c->flags & EK_CFG_ACT8) && (c->w_dtype != EK_I8 || (c->flags & EK_CFG_BLOCK_SCALES)))
         return fail(EK_INVALID_INPUT, "EK_CFG_ACT8 needs w_dtype EK_I8 with one scale per output channel");
-    // 127 * 127 * 131072 < 2^31: the integer sums cannot overflow
     if ((c->flags & EK_CFG_ACT8) && (c->hidden > kAct8MaxK || c->inter > kAct8MaxK))
         return fail(EK_INVALID_INPUT, "EK_CFG_ACT8: hidden and inter must not exceed %lld", (long long)kAct8MaxK);
     if ((c->flags & EK_CFG_BLOCK_SCALES) && c->w_dtype != EK_I8 && c->w_dtype != EK_F8E4M3)

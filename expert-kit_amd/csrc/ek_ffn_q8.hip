@@ -3,8 +3,9 @@
 //
 //   u[n, c] = sum_k q[n, k] w[c, k] * scale[n] * w_scale[c]
 //
-// with the integer sum exact in int32 (|sum| <= 127 * 127 * 131072 < 2^31).  Integer addition is
-// associative, so every split of the contraction and every tile shape below gives the same bits.
+// with the integer sum exact: codes and weights are -128 .. 127 and the contraction at most 131072 long, so the
+// sum lies between -127 * 128 * 131072 and 2^31 = 128 * 128 * 131072.  That one sum does not fit int32; see q8_sum.
+// Integer addition is associative, so every split of the contraction and every tile shape below gives the same bits.
 // Weights lie in HBM as for W8A16 (ek_internal.h): one 1 KiB chunk is the A operand of
 // v_mfma_i32_16x16x64_i8 as it is, but for the offset-binary storage: q = u ^ 0x80.
 #include "ek_internal.h"
@@ -21,6 +22,11 @@ __device__ __forceinline__ i32x4 signed8(uint4 u, uint32_t flip = 0x80808080u)
 {
     return i32x4{(int)(u.x ^ flip), (int)(u.y ^ flip), (int)(u.z ^ flip), (int)(u.w ^ flip)};
 }
+
+// A sum before its conversion to fp32.  Only 2^31 wraps, to the one value that no other sum has; the largest int32
+// becomes 2^31 when it is rounded to fp32.
+constexpr int kQ8WrapChunks = 131072 / 64;       // only the longest contraction can reach it
+__device__ __forceinline__ int q8_sum(int s) { return s == INT32_MIN ? INT32_MAX : s; }
 
 // Four consecutive channels ch .. ch+3 of one output row.
 template <typename T>
@@ -155,6 +161,8 @@ __global__ __launch_bounds__(64 * kQ8Slices) void q8_stream_kernel(Q8Args a, int
             tot[m] = red[0][(rs * NMAT + m) * NG + gi][lane];
 #pragma unroll
             for (int w = 1; w < kQ8Slices; ++w) tot[m] += red[w][(rs * NMAT + m) * NG + gi][lane];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) tot[m][r] = q8_sum(tot[m][r]);
         }
         // lane (g, j) holds channels 4g .. 4g+3 of row j
         const int ch = (nt0 + gi) * 16 + 4 * g;
@@ -415,7 +423,9 @@ typedef const __attribute__((address_space(4))) int32_t *ConstInts;
 typedef const __attribute__((address_space(4))) uint64_t *ConstWords;
 
 // slab_at: the expert's ExpertSlab.  It and the rows' numbers are asked for together.
-template <typename T, int NMAT, int RB>
+// WRAP: sums may be 2^31 (see q8_sum).  They are counted from -1 and the last addition saturates: one operation per sum,
+// in an instance of its own (a selection as q8_sum's spills registers; the ordinary contraction needs neither).
+template <typename T, int NMAT, int RB, bool WRAP>
 __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int row0, int n, int cblock, uint8_t *lds)
 {
     const int tid = threadIdx.x, lane = tid & 63;
@@ -457,7 +467,7 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[rb][cb][r] = 0;
+            for (int r = 0; r < 16; ++r) acc[rb][cb][r] = WRAP ? -1 : 0;
 
     constexpr int D = kQ8Stages;
     uint4 w[D][4][2];
@@ -593,6 +603,7 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int
     const int nch = min(a.N - c0, NC);
     constexpr int PPR = NC / 8;                                  // 16-byte pieces per row
     const bool whole = nch == NC && (a.out_stride & 7) == 0;
+    auto sum_of = [](int v) { return WRAP ? __builtin_elementwise_add_sat(v, 1) : v; };
     // (the lane's number asked for again: kept through the steps it was the one register too many)
     const int elane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
     typedef T T4 __attribute__((ext_vector_type(4)));
@@ -620,13 +631,13 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = q * 4 + r;
-                    v[r] = as_fp32((float)acc[rb][cb][i] * (xs * ws[cb][i]));
+                    v[r] = as_fp32((float)sum_of(acc[rb][cb][i]) * (xs * ws[cb][i]));
                 }
                 T4 o;
                 if constexpr (NMAT == 2) {
                     float gate[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) gate[r] = as_fp32((float)acc[rb][1][q * 4 + r] * (xs * ws[1][q * 4 + r]));
+                    for (int r = 0; r < 4; ++r) gate[r] = as_fp32((float)sum_of(acc[rb][1][q * 4 + r]) * (xs * ws[1][q * 4 + r]));
                     o = swiglu4_rounded<T>(v, gate);
                 } else {
                     if (a.bias) {
@@ -663,7 +674,7 @@ __device__ __forceinline__ void q8_tile(const Q8Args &a, ConstWords slab_at, int
 // Tiles are numbered in groups of `group` items, channel block by channel block within a group; XCD x (workgroups
 // x, x + 8, ...) walks a contiguous eighth of them, so that the workgroups that share an item's rows or an expert's
 // weights run side by side on one L2.
-template <typename T, int NMAT>
+template <typename T, int NMAT, bool WRAP>
 __global__ __launch_bounds__(64 * kQ8Waves, 1) void q8_tile_kernel(Q8Args a, int cblocks, int group)
 {
     extern __shared__ __align__(1024) uint8_t q8_lds[];
@@ -684,14 +695,14 @@ __global__ __launch_bounds__(64 * kQ8Waves, 1) void q8_tile_kernel(Q8Args a, int
     }
     const ConstWords slab = (ConstWords)(uintptr_t)(a.slabs + e);
     switch ((n + 31) >> 5) {
-    case 1: q8_tile<T, NMAT, 1>(a, slab, row0, n, cblock, q8_lds); break;
-    case 2: q8_tile<T, NMAT, 2>(a, slab, row0, n, cblock, q8_lds); break;
-    case 3: q8_tile<T, NMAT, 3>(a, slab, row0, n, cblock, q8_lds); break;
-    case 4: q8_tile<T, NMAT, 4>(a, slab, row0, n, cblock, q8_lds); break;
-    case 5: q8_tile<T, NMAT, 5>(a, slab, row0, n, cblock, q8_lds); break;
-    case 6: q8_tile<T, NMAT, 6>(a, slab, row0, n, cblock, q8_lds); break;
-    case 7: q8_tile<T, NMAT, 7>(a, slab, row0, n, cblock, q8_lds); break;
-    default: q8_tile<T, NMAT, 8>(a, slab, row0, n, cblock, q8_lds); break;
+    case 1: q8_tile<T, NMAT, 1, WRAP>(a, slab, row0, n, cblock, q8_lds); break;
+    case 2: q8_tile<T, NMAT, 2, WRAP>(a, slab, row0, n, cblock, q8_lds); break;
+    case 3: q8_tile<T, NMAT, 3, WRAP>(a, slab, row0, n, cblock, q8_lds); break;
+    case 4: q8_tile<T, NMAT, 4, WRAP>(a, slab, row0, n, cblock, q8_lds); break;
+    case 5: q8_tile<T, NMAT, 5, WRAP>(a, slab, row0, n, cblock, q8_lds); break;
+    case 6: q8_tile<T, NMAT, 6, WRAP>(a, slab, row0, n, cblock, q8_lds); break;
+    case 7: q8_tile<T, NMAT, 7, WRAP>(a, slab, row0, n, cblock, q8_lds); break;
+    default: q8_tile<T, NMAT, 8, WRAP>(a, slab, row0, n, cblock, q8_lds); break;
     }
 }
 
@@ -702,8 +713,11 @@ static hipError_t launch_tiles(const Q8Args &a, int64_t max_items, hipStream_t s
     const int cblocks = (a.NT + per - 1) / per;
     const int64_t tiles = max_items * cblocks, grid = (tiles + 7) / 8 * 8;
     if (grid >= (int64_t)1 << 24) return hipErrorInvalidValue;          // threads of a launch
-    hipLaunchKernelGGL((q8_tile_kernel<T, NMAT>), dim3((unsigned)grid), dim3(64 * kQ8Waves), kQ8Lds, s, a, cblocks,
-                       a.dense_rows > 0 ? 4 : 1);
+    const int group = a.dense_rows > 0 ? 4 : 1;
+    if (a.Kdim >> 6 >= kQ8WrapChunks)
+        hipLaunchKernelGGL((q8_tile_kernel<T, NMAT, true>), dim3((unsigned)grid), dim3(64 * kQ8Waves), kQ8Lds, s, a, cblocks, group);
+    else
+        hipLaunchKernelGGL((q8_tile_kernel<T, NMAT, false>), dim3((unsigned)grid), dim3(64 * kQ8Waves), kQ8Lds, s, a, cblocks, group);
     return hipGetLastError();
 }
 

@@ -308,7 +308,7 @@ ek_status ek_linear_create(const ek_linear_cfg *cfg, const ek_weight_desc *w, co
         if (!cfg) return fail(EK_INVALID_INPUT, "cfg is NULL");
         if (cfg->act_dtype != EK_BF16 && cfg->act_dtype != EK_F16)
             return fail(EK_INVALID_INPUT, "act_dtype must be EK_BF16 or EK_F16 (got %d)", cfg->act_dtype);
-        // 127 * 127 * 131072 < 2^31: the integer sums cannot overflow
+        // 128 * 128 * 131072 = 2^31: the longest contraction whose integer sums the kernels hold (ek_ffn_q8.hip)
         if (cfg->in_features < 1 || cfg->in_features > 131072 || cfg->out_features < 1 || cfg->out_features > (1 << 24))
             return fail(EK_INVALID_INPUT, "in_features (%lld) must be in [1, 131072] and out_features (%lld) in [1, 2^24]",
                         (long long)cfg->in_features, (long long)cfg->out_features);

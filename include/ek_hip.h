@@ -535,10 +535,10 @@ ek_status ek_norm_destroy(ek_norm *norm);
 /* One int8 matrix with a scale per output channel on 8-bit activations (the projections around an MoE
  * block, dense FFN layers):
  *   y[i, c] = rnd16((sum_k q[i, k] w[c, k]) * (x_scale[i] * w_scale[c]) + bias[c])
- * with the sum exact in int32 and the rest in fp32. */
+ * with the sum exact and the rest in fp32. */
 typedef struct ek_linear ek_linear;
 typedef struct ek_linear_cfg {
-    int64_t in_features;   /* 1 .. 131072 (the int32 sums cannot overflow); multiples of 64, at least 128,
+    int64_t in_features;   /* 1 .. 131072 (the integer sums are exact, codes of -128 included); multiples of 64, at least 128,
                               are read where they lie, other lengths through the workspace */
     int64_t out_features;  /* any positive number up to 2^24 */
     int64_t max_rows;      /* largest n a call will pass (sizes the workspace), at most 65535 * 64 */

@@ -57,9 +57,9 @@ struct QuantRow {
         m = tiny ? max_abs * 0x1p64f : max_abs;
         inv = m > 0.f && finite ? 127.f / m : 0.f;
     }
-    // v / 127 for the row's maximum v in the units of what the codes stand for
-    __device__ __forceinline__ float scale_of(float v) const { return finite ? v / 127.f : __builtin_nanf(""); }
-    __device__ __forceinline__ float scale() const { return scale_of(tiny ? m * 0x1p-64f : m); }
+    // m / 127, and v / 127 for the row's maximum v in the units of what the codes stand for: rounded once
+    __device__ __forceinline__ float scale() const { return finite ? (tiny ? m * 0x1p-64f : m) / 127.f : __builtin_nanf(""); }
+    __device__ __forceinline__ float scale_of(double v) const { return finite ? (float)(v * (1.0 / 127.0)) : __builtin_nanf(""); }
     __device__ __forceinline__ uint2 codes(float *p) const
     {
         if (tiny) {

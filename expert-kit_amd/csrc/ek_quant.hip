@@ -132,17 +132,18 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
         }
         const float m = __builtin_bit_cast(float, mb);
         float rstd = 1.f, rlow = 0.f;
+        double root = 1.0;
         if constexpr (NORM) {
             // 1 / sqrt in fp64: the hardware's estimate and one Newton step (relative error below 2^-40), as two fp32
             // values, so that a product with it rounds once
             const double ms = ss * a.inv_h + (double)a.eps;
             const double y0 = __builtin_amdgcn_rsq(ms);
-            const double y1 = y0 * (1.5 - 0.5 * ms * y0 * y0);    // NaN for a row with an infinity or NaN
-            rstd = (float)y1;
-            rlow = (float)(y1 - (double)rstd);
+            root = y0 * (1.5 - 0.5 * ms * y0 * y0);               // NaN for a row with an infinity or NaN
+            rstd = (float)root;
+            rlow = (float)(root - (double)rstd);
         }
         const QuantRow quant(m);
-        if (a.scale && tid == 0) a.scale[row] = NORM ? quant.scale_of(m * rstd) : quant.scale();
+        if (a.scale && tid == 0) a.scale[row] = NORM ? quant.scale_of((double)m * root) : quant.scale();
 
         auto give = [&](int c, float *pv, const V8 &rv) {
             if constexpr (NORM) {

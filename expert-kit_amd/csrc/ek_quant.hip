@@ -5,9 +5,10 @@
 //   m = max|v|,  q = rint(127 v / m) (ties to even),  scale = m / 127;  a row of zeros: q = 0, scale = 0.
 // For the norm, v = p * rstd with p = sum * gain and rstd = 1 / sqrt(mean(sum^2) + eps).  rstd is
 // positive and the same for the whole row, so it cancels out of q: q = rint(127 p / max|p|).
-// p is a product of two 16-bit values, exact in fp32 (at most 22 significant bits), so q is
-// a function of the inputs alone: it does not depend on the order in which the squares are summed,
-// and quant8 (ek_quant.h) gives it exactly, ties included.
+// p is a product of two 16-bit values, exact in fp32 (at most 22 significant bits) as long as it lies in fp32's range
+// (bf16: a product beyond it counts as an infinity, one below 2^-126 loses bits), so q is a function of the inputs
+// alone: it does not depend on the order in which the squares are summed, and quant8 (ek_quant.h) gives it exactly, ties
+// included.
 //
 // Bound: HBM.  A row is read once into registers by one workgroup, which reduces its sum
 // of squares and its maximum together and writes everything from registers: 8192 rows of 7168 with residual and all
@@ -17,6 +18,7 @@
 #include "ek_quant.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ek {
 
@@ -145,14 +147,17 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
         const QuantRow quant(m);
         if (a.scale && tid == 0) a.scale[row] = NORM ? quant.scale_of((double)m * root) : quant.scale();
 
-        auto give = [&](int c, float *pv, const V8 &rv) {
+        auto give = [&](int c, float *pv, const V8 &rv, auto big) {
             if constexpr (NORM) {
                 const int64_t at = row * (a.H >> 3) + c;
                 if (a.sum) ((V8 *)a.sum)[at] = rv;
                 if (a.y) {
                     V8 o;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j] = (T)as_fp32(__builtin_fmaf(pv[j], rstd, pv[j] * rlow));
+                    for (int j = 0; j < 8; ++j) {
+                        const float v = decltype(big)::value ? pv[j] * 0x1p-64f : pv[j];
+                        o[j] = (T)as_fp32(__builtin_fmaf(v, rstd, v * rlow));
+                    }
                     ((V8 *)a.y)[at] = o;
                 }
             }
@@ -161,19 +166,29 @@ __global__ __launch_bounds__(64 * WPR * RPB) void row_quant_kernel(RowQuantArgs 
                 *(uint2 *)(a.q + row * a.q_stride + c * 8) = o;
             }
         };
-        if constexpr (NV > 0) {
+        auto give_row = [&](auto big) {
+            if constexpr (NV > 0) {
 #pragma unroll
-            for (int u = 0; u < NV; ++u) {
-                const int c = u * THREADS + tid;
-                if (c < nvec) give(c, p[u], r[u]);
+                for (int u = 0; u < NV; ++u) {
+                    const int c = u * THREADS + tid;
+                    if (c < nvec) give(c, p[u], r[u], big);
+                }
+            } else {
+                for (int c = tid; c < nvec; c += THREADS) {
+                    RawCols<T, MODE> raw;
+                    raw.load(a, row, c, nvec);
+                    r[0] = raw.values(c, a.H, p[0]);
+                    give(c, p[0], r[0], big);
+                }
             }
+        };
+        if (NORM && std::is_same<T, __bf16>::value && rstd < 0x1p-100f) {
+            // a row of values beyond 2^100: fp32 would not hold the root's low part, nor at the range's end the root itself
+            rstd = (float)(root * 0x1p64);
+            rlow = (float)(root * 0x1p64 - (double)rstd);
+            give_row(std::true_type{});
         } else {
-            for (int c = tid; c < nvec; c += THREADS) {
-                RawCols<T, MODE> raw;
-                raw.load(a, row, c, nvec);
-                r[0] = raw.values(c, a.H, p[0]);
-                give(c, p[0], r[0]);
-            }
+            give_row(std::false_type{});
         }
         // the padding of an int8 row that the products read in whole steps
         if (a.q)

@@ -34,3 +34,37 @@ def test_scale_is_rounded_once(ek, cuda, dt, n, H):
         # the reciprocal root is within 2^-40 and two fp64 products follow: 2^-15 of a half step
         worst = float(scale_error(out, x, res, gain).max())
         assert worst <= 1.0 + 2.0 ** -14, f"{worst} half steps"
+
+
+@pytest.mark.parametrize("n,H", [(4, 72), (300, 1000), (400, 7168), (30, 16384), (9, 33000)])
+@pytest.mark.parametrize("magnitude", [2.0 ** 100, 2.0 ** 112, 2.0 ** 120, 2.0 ** 125])
+def test_rows_near_the_types_largest_values(ek, cuda, n, H, magnitude):
+    """bf16 rows whose reciprocal root is near fp32's smallest normal number, or below it: y as at any other magnitude."""
+    dt = torch.bfloat16
+    x, r, gain = make(n, H, dt, seed=2, scale=magnitude)
+    gain = (gain.float() * 2.0 ** -9).to(dt)                           # sum * gain within fp32's range
+    out = ek.HipNorm(gain).forward(x.to(cuda), r.to(cuda))
+    total, v, q, s = ref.norm(x, r, gain, EPS)
+    assert bool(total.isfinite().all()) and torch.equal(out.sum.cpu(), total) and torch.equal(out.q.cpu().double(), q)
+    assert float(scale_error(out, x, r, gain).max()) <= 1.0 + 2.0 ** -14
+    low, high = (v * (1 - 2.0 ** -38)).float().to(dt), (v * (1 + 2.0 ** -38)).float().to(dt)
+    clear, y = low == high, out.y.cpu()                                # away from a border of fp32 the answer is one
+    assert int((~clear).sum()) <= 8
+    wrong = int((y[clear] != low[clear]).sum())
+    assert wrong == 0, f"{wrong} of {y.numel()}"
+
+
+def test_largest_rows_of_all(ek, cuda):
+    """Rows that hold bf16's largest values only: the mean of squares is beyond fp32 and the root at its end."""
+    dt, H = torch.bfloat16, 640
+    big = torch.finfo(dt).max
+    g = torch.Generator().manual_seed(3)
+    x = torch.where(torch.rand(20, H, generator=g) < 0.5, -big, big).to(dt)
+    x[10:] = (x[10:].float() * (0.5 + 0.5 * torch.rand(10, H, generator=g))).to(dt)
+    gain = (0.25 + 0.5 * torch.rand(H, generator=g)).to(dt)
+    out = ek.HipNorm(gain).forward(x.to(cuda))
+    _, v, q, _ = ref.norm(x, None, gain, EPS)
+    assert torch.equal(out.q.cpu().double(), q) and float(scale_error(out, x, None, gain).max()) <= 1.0 + 2.0 ** -14
+    low, high = (v * (1 - 2.0 ** -38)).float().to(dt), (v * (1 + 2.0 ** -38)).float().to(dt)
+    clear = low == high
+    assert torch.equal(out.y.cpu()[clear], low[clear])

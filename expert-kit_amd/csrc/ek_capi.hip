@@ -1579,7 +1579,8 @@ ek_status ek_layer_forward_q8(ek_layer *layer, const void *x, const float *x_sca
         if (!layer) return fail(EK_INVALID_INPUT, "layer is NULL");
         if (!layer->act8) return fail(EK_INVALID_INPUT, "8-bit rows need a layer created with EK_CFG_ACT8");
         if (T > 0 && !x_scale) return fail(EK_INVALID_INPUT, "NULL tensor pointer");
-        if (mem == EK_DEVICE && (((uintptr_t)x & 15) || ((uintptr_t)x_scale & 3)))
+        // (a padded layer copies the rows byte by byte)
+        if (mem == EK_DEVICE && ((!layer->padded && ((uintptr_t)x & 15)) || ((uintptr_t)x_scale & 3)))
             return fail(EK_INVALID_INPUT, "8-bit rows must be 16-byte aligned, their scales 4-byte aligned");
         return layer_forward(layer, x, x_scale, ids, w, w_dtype, T, y, route, mem, stream);
     )

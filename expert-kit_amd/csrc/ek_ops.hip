@@ -171,7 +171,7 @@ ek_status enqueue_linear(ek_linear *L, const void *x, const float *x_scale, int6
     if (!x_scale) {
         ek::RowQuantArgs r{};
         r.x = x; r.q = L->wq; r.scale = L->ws; r.n = n; r.H = (int32_t)K; r.q_stride = (int32_t)L->Kp;
-        r.vec = K % 8 == 0;
+        r.vec = K % 8 == 0 && !misaligned(x, 16);
         EK_HIP(ek::launch_row_quant(r, L->act, false, s));
         a.x = L->wq;
         a.x_scale = L->ws;
@@ -357,8 +357,10 @@ ek_status ek_linear_forward(ek_linear *linear, const void *x, const float *x_sca
         DeviceGuard dg(linear->cfg.device_id);
         if (!dg.ok) return fail(EK_HIP_ERROR, "hipSetDevice(%d) failed", linear->cfg.device_id);
         if (mem == EK_DEVICE) {
-            if (misaligned(x, 16) || misaligned(y, 16) || misaligned(x_scale, 4))
-                return fail(EK_INVALID_INPUT, "device tensors must be 16-byte aligned (x_scale: 4)");
+            // rows read in place go 16 bytes at a time, others by their elements; y is written in pieces that its rows' length allows
+            const uintptr_t x_to = !own_rows ? 16 : x_scale ? 1 : 2, y_to = N % 8 == 0 ? 16 : N % 4 == 0 ? 8 : 2;
+            if (misaligned(x, x_to) || misaligned(y, y_to) || misaligned(x_scale, 4))
+                return fail(EK_INVALID_INPUT, "device tensors must be aligned: x to %d bytes, y to %d, x_scale to 4", (int)x_to, (int)y_to);
             if (stream && !own_rows) return enqueue_linear(linear, x, x_scale, n, y, (hipStream_t)stream);
             std::lock_guard<std::mutex> lk(linear->mu);
             hipStream_t s = stream ? (hipStream_t)stream : linear->stream;

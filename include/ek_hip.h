@@ -230,7 +230,8 @@ ek_status ek_layer_forward(ek_layer *layer, const void *x, const int32_t *ids, c
                            int32_t mem, void *stream);
 
 /* ek_layer_forward on rows that are 8-bit already (ek_norm_forward's q and scale): x [T, hidden] int8,
- * x_scale [T] fp32; on the device x is 16-byte and x_scale 4-byte aligned.  The layer was created with
+ * x_scale [T] fp32; on the device x is 16-byte aligned (where the layer's hidden and inter are multiples of 64, at least
+ * 128; other layers copy the rows) and x_scale 4-byte aligned.  The layer was created with
  * EK_CFG_ACT8; everything else as in ek_layer_forward, and the same bits as its call on 16-bit rows whose
  * quantisation is (x, x_scale). */
 ek_status ek_layer_forward_q8(ek_layer *layer, const void *x, const float *x_scale, const int32_t *ids, const void *w,
@@ -550,7 +551,9 @@ typedef struct ek_linear_cfg {
  * (EK_BF16, EK_F16, EK_F32), in w->mem, or NULL. */
 ek_status ek_linear_create(const ek_linear_cfg *cfg, const ek_weight_desc *w, const void *bias, int32_t bias_dtype, ek_linear **out);
 /* x [n, in_features] int8 with x_scale [n], or of act_dtype with x_scale NULL (the library quantises the
- * rows first) -> y [n, out_features].  Device tensors are 16-byte aligned.  Calls that go through the
+ * rows first) -> y [n, out_features].  On the device 8-bit rows of a length read in place are 16-byte aligned, other rows as
+ * their elements; y to 16 bytes where out_features is a multiple of 8, to 8 where it is one of 4, else to 2 (so that
+ * any slice of whole rows serves); x_scale to 4.  Calls that go through the
  * workspace are ordered on the device like a layer's; the others share nothing and may overlap. */
 ek_status ek_linear_forward(ek_linear *linear, const void *x, const float *x_scale, int64_t n, void *y, int32_t mem, void *stream);
 ek_status ek_linear_shape(ek_linear *linear, int64_t *in_features, int64_t *out_features);

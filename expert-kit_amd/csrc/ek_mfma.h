@@ -172,10 +172,11 @@ template <typename T> __device__ __forceinline__ T swiglu_rounded(float acc_up, 
 }
 
 // Four elements of swiglu_rounded at once, the same bits.  silu comes from the hardware's exp2 and reciprocal and stands
-// where its storage rounding cannot fall the other way: not within two fp32 steps of a tie, with a result that is a normal
-// number of T and |gate| < 64.  Otherwise the lane takes the form above.  What the two forms differ by was listed for
-// all 65536 values of either type: one gate of each type rounds differently, from a tie or one step off it (and a test
-// compares all of them).  With random gates a wave of 256 elements takes the long form in 2 of 100 cases (bf16) or 14 (fp16).
+// when it is not within two fp32 steps of a tie of its storage rounding, is a normal number of T, and |gate| < 64;
+// otherwise the lane takes the form above.  No error bound says that two steps suffice (near |gate| = 60 the product with
+// log2 e alone is off by tens of steps): gate has 65536 values of either type, silu depends on nothing else, and on gfx950
+// the two forms were compared for every one of them.  One gate of each type rounds differently, from a tie or one step
+// off it, and the guard covers both; test_every_gate_value compares them all through the kernels.  With random gates a wave of 256 elements takes the long form in 2 of 100 cases (bf16) or 14 (fp16).
 // Used where a wave has nothing to hide the arithmetic behind (the epilogue of the int8 tile kernel, one wave per SIMD):
 // 5057 tokens, 128 experts of 2048 x 768, top-8: 480 -> 467 us; 8192 tokens, 256 of 7168 x 2048: 4285 -> 4238 us (MI355X).
 template <typename T> struct T4Of { typedef T type __attribute__((ext_vector_type(4))); };

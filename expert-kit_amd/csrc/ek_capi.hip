@@ -1809,25 +1809,25 @@ ek_status ek_layer_experts_forward(ek_layer *layer, int32_t n_calls, const int32
             // Work lists cut on the host exactly as the pack kernels cut them: a call is one
             // segment (ek_internal.h, "work lists").
             std::vector<ek::WorkItem> items[ek::kNumLists];
-            int64_t row0 = 0, tile_items = 0, wide_items = 0, short_items = 0, q8_tiles = 0, q8_rows = 0, longest = 0;
+            int64_t row0 = 0, tile_items = 0, wide_items = 0, short_items = 0;
+            ek::Q8Batch q8;
             for (int i = 0; i < n_calls; ++i) {
                 tile_items += (rows[i] >> 7) + ((rows[i] & 127) > 16);
                 wide_items += (rows[i] + ek::kWideRows - 1) / ek::kWideRows;
                 short_items += (rows[i] & 127) > 0 && (rows[i] & 127) <= 16;
-                if (rows[i] > 16) { q8_tiles += ek::q8_items((int)rows[i]); q8_rows += rows[i]; }
-                longest = std::max(longest, rows[i]);
+                q8.add(rows[i]);
             }
             // The wide cut spares a batch the tile kernel's long, nearly empty launch.  When the batch
             // also has many short requests, their streaming chain (one pass over an expert's weights
             // each, ~6.5 TB/s) runs beside the tile chain and covers it, and the short items are
             // served faster by the sliced streaming form than by the wide one (64 DeepSeek-V3 int8
             // requests from host memory, 4 rows each but one of 40 / four of 100: 995 / 1500 us cut wide,
-            // 890 / 1325 us as tiles beside streams).
+            // 890 / 1325 us as tiles beside streams).  (8-bit activations: see ek::Q8Batch.)
             const int wb = layer->w8 ? 1 : 2;
             const double cover_us = (double)short_items * 3.0 * (double)H * (double)layer->cfg.inter * wb / 6.5e6;
             const double tiled_us = ek::tile_call_us(H, layer->cfg.inter);
-            const bool wide = (layer->act8 ? ek::q8_wide_cut_pays(q8_rows, q8_tiles, longest, H, layer->cfg.inter)
-                                           : ek::wide_cut_pays(tile_items, P, H, layer->cfg.inter)) && cover_us < 0.5 * tiled_us &&
+            const bool wide = (layer->act8 ? q8.streamed(H, layer->cfg.inter)
+                                           : ek::wide_cut_pays(tile_items, P, H, layer->cfg.inter) && cover_us < 0.5 * tiled_us) &&
                               wide_items <= layer->ws.list_cap[ek::kListStream];
             for (int i = 0; i < n_calls; ++i) {
                 const int32_t n = (int32_t)rows[i], full = n >> 7, r = n & 127;

@@ -122,8 +122,8 @@ inline double q8_tiles_us(int64_t items, int64_t item_rows, int64_t K, int64_t N
     return (double)rounds * (14.0 + (double)(K + 127) / 128.0 * (0.45 + 0.1 * blocks));
 }
 inline double q8_tile_us(int64_t n, int64_t K, int64_t N) { return q8_tiles_us((n + kQ8Rows - 1) / kQ8Rows, n, K, N); }
-// Per-expert calls: rows in all, and how many tile items of at most item_rows rows they would be: whether both stages
-// are better streamed.
+// One expert's call: its rows, and how many tile items of at most item_rows rows they would be: whether both stages are
+// better streamed.
 inline bool q8_wide_cut_pays(int64_t rows, int64_t items, int64_t item_rows, int64_t hidden, int64_t inter)
 {
     return items > 0 && q8_stream_us(rows, hidden, 2 * inter) + q8_stream_us(rows, inter, hidden) <
@@ -131,6 +131,34 @@ inline bool q8_wide_cut_pays(int64_t rows, int64_t items, int64_t item_rows, int
 }
 // Item i of the one-class cut of a segment of n rows (n > 16) into `items`: its first row and its rows.
 constexpr int q8_items(int n) { return (n + kQ8Rows - 1) / kQ8Rows; }
+// A grouped launch of several experts' calls: either all of them streamed in items of up to kWideRows rows, or those
+// of more than 16 rows as tiles behind a streaming launch of the others (a stage's two launches run in turn).  Streaming
+// reads an expert's weights once per 32 rows, at 6.5 TB/s whatever the products take, and costs a short call 9 % more than
+// the short form.  Measured on MI355X, each launch on other experts than the one before, streamed / tiles beside streams, us:
+//   7168 x 2048:  1 call of 40 rows 48 / 82, 1 of 500 102 / 152, 4 of 20 80 / 99, 4 of 100 168 / 146, 16 of 40 318 / 198;
+//                 16 calls of 1 row with one of 200 267 / 310, with 4 of 100 285 / 253; 40 calls of 8 rows with one of 20 357 / 372
+//   2048 x 768:   1 call of 40 rows 35 / 45, 4 of 100 61 / 78, 16 of 40 71 / 71; 40 calls of 8 rows with one of 200 108 / 148
+struct Q8Batch {
+    int64_t shorts = 0;                                          // calls of up to 16 rows
+    int64_t rows = 0, tiles = 0, longest = 0, passes = 0;        // of the others
+    void add(int64_t n)
+    {
+        if (n <= 16) { shorts += n > 0; return; }
+        rows += n;
+        tiles += q8_items((int)n);
+        longest = n > longest ? n : longest;
+        passes += n / kWideRows * (kWideRows / 32) + (n % kWideRows + 31) / 32;
+    }
+    bool streamed(int64_t hidden, int64_t inter) const
+    {
+        if (rows == 0) return false;
+        const double weights_us = 3.0 * (double)hidden * (double)inter / 6.5e6;
+        const double products = q8_stream_us(rows, hidden, 2 * inter) + q8_stream_us(rows, inter, hidden);
+        const double reads = (double)passes * weights_us;
+        return (products > reads ? products : reads) + 0.09 * (double)shorts * weights_us <
+               q8_tiles_us(tiles, longest, hidden, 2 * inter) + q8_tiles_us(tiles, longest, inter, hidden);
+    }
+};
 __host__ __device__ inline void q8_item(int n, int items, int i, int *first, int *rows)
 {
     const int blocks = (n + 31) >> 5, base = blocks / items, more = blocks % items;

@@ -1144,9 +1144,14 @@ SharedCut shared_cut(const ek_layer *L, int64_t T)
 {
     SharedCut c;
     c.shared = L->expert_mem[L->cfg.n_experts] != nullptr && T > 0;
-    c.streamed = c.shared && T <= kSharedStreamRows;
-    c.wide = c.shared && !c.streamed && T <= kSharedWideRows;
     c.own = c.shared && L->shared_inter != 0;
+    // On 8-bit activations a segment with launches of its own is cut wide from the first row on (64 experts of 7168 x 2048
+    // beside a shared one of 4096, 8 / 32 / 64 tokens: 324 / 464 / 509 us, in 16-row items 329 / 485 / 552; 128 of 2048 x 768
+    // beside 1536: 82 / 125 / 139, 83 / 126 / 143).  In the routed pairs' list 16-row items stay better or equal up to
+    // kSharedStreamRows: a wide cut is a launch more (the same layers beside a shared expert of their own width, 64 tokens:
+    // 512 against 506 us, 126 against 136).
+    c.streamed = c.shared && T <= kSharedStreamRows && !(L->act8 && c.own);
+    c.wide = c.shared && !c.streamed && T <= kSharedWideRows;
     return c;
 }
 

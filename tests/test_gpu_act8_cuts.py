@@ -70,6 +70,20 @@ def test_large_layer_with_a_shared_expert(ek, cuda, T, K, cls, width):
     both(lay, x, ids, w, ref.layer(*ref.quantise(x), ids, w, ws, dt, shared), cuda, f"{T} tokens, top-{K}, shared {width * I}")
 
 
+@pytest.mark.parametrize("T,K,cls", [(2, 4, 1), (40, 4, 1), (200, 2, 1), (300, 4, 2)])
+def test_tokens_that_name_an_expert_twice(ek, cuda, T, K, cls):
+    """Routings drawn with replacement, among them tokens whose pairs are all of one expert."""
+    dt = torch.float16
+    check_class(T, K, cls)
+    lay, ws, shared = layer(ek, K, dt, shared_inter=I, seed=9)
+    x, _, w = call(T, H, E, K, dt, seed=T + 9, w32=True)
+    g = torch.Generator().manual_seed(T)
+    ids = torch.randint(0, E, (T, K), generator=g).to(torch.int32)
+    ids[:: 3] = ids[:: 3, :1]
+    ids[1::4] = 7
+    both(lay, x, ids, w, ref.layer(*ref.quantise(x), ids, w, ws, dt, shared), cuda, f"{T} tokens, top-{K}")
+
+
 @pytest.mark.parametrize("shared_inter", [None, I, 2 * I])
 @pytest.mark.parametrize("T,K,cls", [(64, 2, 1), (96, 4, 1), (200, 4, 2)])
 def test_static_workspace(ek, cuda, T, K, cls, shared_inter):

@@ -392,8 +392,9 @@ __global__ __launch_bounds__(64 * (kPairDirectMaxK + 1)) void q8_pairs_down_kern
 // what the one and 60 % of what the other can.  (128 rows per wave, two workgroups per CU, wants 96 KiB of the L1: it was
 // the bound.  8192 x 8192 x 8192 on MI355X: 1.84 POP/s, and 2.73 with the weight loads taken out.)
 // Measured on MI355X: that product 468 us = 2.35 POP/s; 8192 tokens of 256 experts of 7168 x 2048, top-8: 2.3 + 1.5 ms, the
-// matrix pipes busy for 44 and 36 % of the cycles at 1.8 GHz.  A step costs 1.3 to 1.7 us, and ~14 us of a tile are
-// its start, its epilogue and its stores, which is what bounds short contractions (768: two thirds of the time).
+// matrix pipes busy for 44 and 36 % of the cycles at 1.8 GHz.  With 256 tiles of 256
+// rows at once a step takes 1.7 us and a tile 16 us beside its steps (launch, first loads, conversion, stores), 21 with SwiGLU, which
+// is what bounds short contractions (768: two thirds of the time).
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __forceinline__ void dma16(const void *gaddr, uint32_t lds_addr)     // lane l's 16 bytes land at lds_addr + 16 l

@@ -138,6 +138,7 @@ constexpr int q8_items(int n) { return (n + kQ8Rows - 1) / kQ8Rows; }
 //   7168 x 2048:  1 call of 40 rows 48 / 82, 1 of 500 102 / 152, 4 of 20 80 / 99, 4 of 100 168 / 146, 16 of 40 318 / 198;
 //                 16 calls of 1 row with one of 200 267 / 310, with 4 of 100 285 / 253; 40 calls of 8 rows with one of 20 357 / 372
 //   2048 x 768:   1 call of 40 rows 35 / 45, 4 of 100 61 / 78, 16 of 40 71 / 71; 40 calls of 8 rows with one of 200 108 / 148
+// Of 119 drawn batches on four shapes (1024 x 512 to 7168 x 2048) the rule took the form more than 5 % slower in none.
 struct Q8Batch {
     int64_t shorts = 0;                                          // calls of up to 16 rows
     int64_t rows = 0, tiles = 0, longest = 0, passes = 0;        // of the others
